@@ -105,7 +105,8 @@ typedef struct rs_plan rs_plan;
 typedef struct rs_program rs_program;
 
 const char* rs_last_error(void);
-/* 1.1 adds rs_copy_launch_noalloc, rs_act_plan and rs_act_resolve; 1.2 adds rs_copy_run_bounded.
+/* 1.1 adds rs_copy_launch_noalloc, rs_act_plan and rs_act_resolve; 1.2 adds rs_copy_run_bounded;
+ * 1.3 adds the training-step operators.
  * The 1.0 entry points are unchanged. */
 int rs_version(int32_t* major, int32_t* minor);
 
@@ -416,6 +417,121 @@ int rs_act_resolve(const rs_stage_mesh* src, const rs_stage_mesh* dst, const rs_
                    const rs_act_piece* pieces, int64_t n_pieces,
                    const uint64_t* src_dev, const uint64_t* dst_dev, int32_t n_ranks,
                    rs_copy_desc* out, int64_t capacity, int64_t* n_out);
+
+/* ---- the training step on a rank's shards ----------------------------------------------- */
+/* Operators that run on the state these layouts move: gradient norm and clipping, the AdamW update of
+ * a rank's sub-fields, lookup and gradient of an embedding's vocabulary shard, log probabilities of a
+ * lm_head shard's logits. Every entry launches on `stream` of `device` (any device may be current),
+ * allocates nothing, waits for nothing and keeps nothing, so it can be captured into a CUDA graph.
+ * Results do not depend on the order in which CTAs run. Workspaces are the caller's; calls that may run at the
+ * same time need a workspace each. Element types: */
+enum rs_dtype { RS_F32 = 0, RS_BF16 = 1, RS_F16 = 2 };
+
+/* One dense run of gradient elements that this rank counts. */
+typedef struct rs_grad_span {
+  uint64_t grad_dev;
+  uint64_t numel;
+  uint32_t dtype;
+  uint32_t reserved;
+} rs_grad_span;
+
+/* *sumsq_dev = sum of squares over the spans (0 for none), summed in 64 bits. */
+int rs_grad_sumsq_workspace_bytes(int64_t n_spans, uint64_t* bytes);
+int rs_grad_sumsq(const rs_grad_span* spans, int64_t n_spans, void* workspace_dev, uint64_t workspace_bytes,
+                  double* sumsq_dev, int32_t device, void* stream);
+
+/* norm = sqrt(*sumsq_dev) -> *norm_dev; every element of the spans times min(1, max_norm / (norm + 1e-6)).
+ * *sumsq_dev may have been reduced over ranks since rs_grad_sumsq wrote it. Spans must not overlap. */
+int rs_grad_clip(const rs_grad_span* spans, int64_t n_spans, const double* sumsq_dev, float max_norm, float* norm_dev,
+                 int32_t device, void* stream);
+
+/* One tensor's sub-fields. With a master copy (fp32) the update runs on it and param gets it rounded; without
+ * (master_dev 0) it runs on param. grad and param: any rs_dtype; moments: RS_F32 or RS_BF16; step: one fp32. */
+typedef struct rs_adamw_tensor {
+  uint64_t grad_dev;
+  uint64_t param_dev;
+  uint64_t master_dev;
+  uint64_t exp_avg_dev;
+  uint64_t exp_avg_sq_dev;
+  uint64_t step_dev;
+  uint64_t numel;
+  float weight_decay;
+  uint32_t grad_dtype;
+  uint32_t param_dtype;
+  uint32_t moment_dtype;
+} rs_adamw_tensor;
+
+typedef struct rs_adamw_opts {
+  double lr;
+  double beta1;
+  double beta2;
+  double eps;
+  double max_norm; /* used when sumsq_dev is given */
+} rs_adamw_opts;
+
+/* step += 1 and one AdamW update of every tensor. sumsq_dev (or NULL: no clipping): the gradients count
+ * times min(1, max_norm / (sqrt(*sumsq_dev) + 1e-6)) without being written, and the norm goes to norm_dev
+ * (may be NULL). No two tensors may share memory. */
+int rs_adamw_workspace_bytes(int64_t n_tensors, uint64_t* bytes);
+int rs_adamw_step(const rs_adamw_tensor* tensors, int64_t n_tensors, const rs_adamw_opts* opts, const double* sumsq_dev,
+                  float* norm_dev, void* workspace_dev, uint64_t workspace_bytes, int32_t device, void* stream);
+
+/* An embedding's vocabulary shard: rows [lo, lo + rows) of the whole table. */
+typedef struct rs_embed_opts {
+  int64_t n_tokens;
+  int64_t rows;
+  int64_t hidden;
+  int64_t lo;
+  int64_t weight_stride;  /* elements between rows of the weight (lookup) */
+  int64_t grad_stride;    /* elements between rows of the output's gradient (gradient) */
+  float scale;
+  uint32_t dtype;         /* of weight, output and the output's gradient */
+  uint32_t grad_dtype;    /* of the weight's gradient */
+  int32_t wide_ids;       /* ids are int64, else int32 */
+  int32_t accumulate;     /* add to the gradient that is there, else write all rows of it */
+  int32_t reserved;
+} rs_embed_opts;
+
+/* out[i] = scale * weight[ids[i] - lo], zeros for an id that the shard does not hold; out is contiguous. */
+int rs_embed_lookup(const rs_embed_opts* opts, const void* ids_dev, const void* weight_dev, void* out_dev, int32_t device,
+                    void* stream);
+/* grad[r] (+)= scale * sum of grad_out[i] over the tokens whose id is lo + r, in 32 bits; grad is contiguous
+ * [rows, hidden]. At most 65536 tokens (RS_ERR_CAPACITY). */
+int rs_embed_grad_workspace_bytes(const rs_embed_opts* opts, int32_t device, uint64_t* bytes);
+int rs_embed_grad(const rs_embed_opts* opts, const void* ids_dev, const void* grad_out_dev, void* grad_dev,
+                  void* workspace_dev, uint64_t workspace_bytes, int32_t device, void* stream);
+
+/* Logits [n_rows, cols] of vocabulary indices [lo, lo + cols); rows `stride` elements apart. */
+typedef struct rs_logprob_opts {
+  int64_t n_rows;
+  int64_t cols;
+  int64_t stride;
+  int64_t lo;
+  uint32_t dtype;
+  int32_t wide_targets;   /* targets are int64, else int32 */
+  int32_t top;            /* alternatives, 0..32 */
+  int32_t sharded;        /* gradient: a target outside the shard is another shard's, else it is no target */
+} rs_logprob_opts;
+
+/* Per row: log probability of the target (0 where the target is in no shard), entropy, log-sum-exp, and the
+ * `top` largest logits' log probabilities and vocabulary indices, largest first, ties to the lowest index
+ * (index -1 and log probability -inf where there are fewer). A row of -inf alone has lse and log probabilities -inf and entropy 0. */
+int rs_token_logprobs(const rs_logprob_opts* opts, const void* logits_dev, const void* targets_dev, float* logprob_dev,
+                      float* entropy_dev, float* lse_dev, float* top_logprob_dev, int64_t* top_index_dev, int32_t device,
+                      void* stream);
+/* The same for one shard of several: a record of 4 + 2 top floats per row, and the join of all shards' records,
+ * [n_shards][n_rows][4 + 2 top] with shards in ascending order of their first index, starts[s] (host
+ * memory; at most 64 shards). */
+int rs_token_record(const rs_logprob_opts* opts, const void* logits_dev, const void* targets_dev, float* record_dev,
+                    int32_t device, void* stream);
+int rs_token_merge(const float* records_dev, const int64_t* starts, int32_t n_shards, int64_t n_rows, int32_t top,
+                   float* logprob_dev, float* entropy_dev, float* lse_dev, float* top_logprob_dev, int64_t* top_index_dev,
+                   int32_t device, void* stream);
+/* d logits of sum(grad_logprob * logprob) + sum(grad_entropy * entropy) + sum(grad_lse * lse); grad_entropy_dev and
+ * grad_lse_dev may be NULL, grad_dev may be the logits. lse and entropy are those of the whole vocabulary. A row of -inf alone has gradient 0. */
+int rs_token_logprobs_grad(const rs_logprob_opts* opts, const void* logits_dev, const void* targets_dev, const float* lse_dev,
+                           const float* entropy_dev, const float* grad_logprob_dev, const float* grad_entropy_dev,
+                           const float* grad_lse_dev, void* grad_dev, int64_t grad_stride, int32_t device, void* stream);
 
 #ifdef __cplusplus
 }

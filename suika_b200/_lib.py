@@ -130,6 +130,34 @@ class RsActGeometry(C.Structure):
                 ("shape", C.c_int64 * RS_MAX_DIMS)]
 
 
+RS_F32, RS_BF16, RS_F16 = 0, 1, 2
+
+
+class RsGradSpan(C.Structure):
+    _fields_ = [("grad_dev", C.c_uint64), ("numel", C.c_uint64), ("dtype", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class RsAdamwTensor(C.Structure):
+    _fields_ = [("grad_dev", C.c_uint64), ("param_dev", C.c_uint64), ("master_dev", C.c_uint64), ("exp_avg_dev", C.c_uint64),
+                ("exp_avg_sq_dev", C.c_uint64), ("step_dev", C.c_uint64), ("numel", C.c_uint64), ("weight_decay", C.c_float),
+                ("grad_dtype", C.c_uint32), ("param_dtype", C.c_uint32), ("moment_dtype", C.c_uint32)]
+
+
+class RsAdamwOpts(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("max_norm", C.c_double)]
+
+
+class RsEmbedOpts(C.Structure):
+    _fields_ = [("n_tokens", C.c_int64), ("rows", C.c_int64), ("hidden", C.c_int64), ("lo", C.c_int64),
+                ("weight_stride", C.c_int64), ("grad_stride", C.c_int64), ("scale", C.c_float), ("dtype", C.c_uint32),
+                ("grad_dtype", C.c_uint32), ("wide_ids", C.c_int32), ("accumulate", C.c_int32), ("reserved", C.c_int32)]
+
+
+class RsLogprobOpts(C.Structure):
+    _fields_ = [("n_rows", C.c_int64), ("cols", C.c_int64), ("stride", C.c_int64), ("lo", C.c_int64), ("dtype", C.c_uint32),
+                ("wide_targets", C.c_int32), ("top", C.c_int32), ("sharded", C.c_int32)]
+
+
 # numpy mirrors used to fill large descriptor arrays without a Python loop per field.
 TENSOR_META_DTYPE = np.dtype([("name_id", "<i4"), ("ndim", "<i4"), ("shape", "<i8", (RS_MAX_DIMS,)),
                               ("itemsize", "<i4"), ("slice_dim", "<i4"), ("tp_index", "<i4"), ("tp_deg", "<i4")])
@@ -139,6 +167,12 @@ SEGMENT_DTYPE = np.dtype([("src_slot", "<i4"), ("dst_slot", "<i4"), ("src_offset
                           ("rows", "<u8"), ("row_bytes", "<u8"), ("src_pitch", "<u8"), ("dst_pitch", "<u8")])
 ACT_PIECE_DTYPE = np.dtype([("src_rank", "<i4"), ("dst_rank", "<i4"), ("src_batch", "<i8"), ("dst_batch", "<i8"),
                             ("n_batch", "<i8"), ("slice_start", "<i8"), ("slice_len", "<i8")])
+GRAD_SPAN_DTYPE = np.dtype([("grad_dev", "<u8"), ("numel", "<u8"), ("dtype", "<u4"), ("reserved", "<u4")])
+ADAMW_TENSOR_DTYPE = np.dtype([("grad_dev", "<u8"), ("param_dev", "<u8"), ("master_dev", "<u8"), ("exp_avg_dev", "<u8"),
+                               ("exp_avg_sq_dev", "<u8"), ("step_dev", "<u8"), ("numel", "<u8"), ("weight_decay", "<f4"),
+                               ("grad_dtype", "<u4"), ("param_dtype", "<u4"), ("moment_dtype", "<u4")])
+assert GRAD_SPAN_DTYPE.itemsize == C.sizeof(RsGradSpan)
+assert ADAMW_TENSOR_DTYPE.itemsize == C.sizeof(RsAdamwTensor)
 assert TENSOR_META_DTYPE.itemsize == C.sizeof(RsTensorMeta)
 assert ACT_PIECE_DTYPE.itemsize == C.sizeof(RsActPiece)
 assert COPY_DESC_DTYPE.itemsize == C.sizeof(RsCopyDesc)
@@ -180,6 +214,18 @@ SIGNATURES = {
                               C.POINTER(C.c_int64)]),
     "rs_act_resolve": (C.c_int, [C.POINTER(RsStageMesh), C.POINTER(RsStageMesh), C.POINTER(RsActGeometry), _P, C.c_int64,
                                  _P, _P, C.c_int32, _P, C.c_int64, C.POINTER(C.c_int64)]),
+    "rs_grad_sumsq_workspace_bytes": (C.c_int, [C.c_int64, C.POINTER(C.c_uint64)]),
+    "rs_grad_sumsq": (C.c_int, [_P, C.c_int64, _P, C.c_uint64, _P, C.c_int32, _P]),
+    "rs_grad_clip": (C.c_int, [_P, C.c_int64, _P, C.c_float, _P, C.c_int32, _P]),
+    "rs_adamw_workspace_bytes": (C.c_int, [C.c_int64, C.POINTER(C.c_uint64)]),
+    "rs_adamw_step": (C.c_int, [_P, C.c_int64, C.POINTER(RsAdamwOpts), _P, _P, _P, C.c_uint64, C.c_int32, _P]),
+    "rs_embed_lookup": (C.c_int, [C.POINTER(RsEmbedOpts), _P, _P, _P, C.c_int32, _P]),
+    "rs_embed_grad_workspace_bytes": (C.c_int, [C.POINTER(RsEmbedOpts), C.c_int32, C.POINTER(C.c_uint64)]),
+    "rs_embed_grad": (C.c_int, [C.POINTER(RsEmbedOpts), _P, _P, _P, _P, C.c_uint64, C.c_int32, _P]),
+    "rs_token_logprobs": (C.c_int, [C.POINTER(RsLogprobOpts), _P, _P, _P, _P, _P, _P, _P, C.c_int32, _P]),
+    "rs_token_record": (C.c_int, [C.POINTER(RsLogprobOpts), _P, _P, _P, C.c_int32, _P]),
+    "rs_token_merge": (C.c_int, [_P, _P, C.c_int32, C.c_int64, C.c_int32, _P, _P, _P, _P, _P, C.c_int32, _P]),
+    "rs_token_logprobs_grad": (C.c_int, [C.POINTER(RsLogprobOpts), _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, C.c_int32, _P]),
 }
 
 _lock = threading.Lock()

@@ -15,8 +15,8 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libsuika_reshard.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = [os.path.join(CSRC, "plan.cpp"), os.path.join(CSRC, "act.cpp"), os.path.join(CSRC, "exec.cu")]
-DEPS = SOURCES + [os.path.join(CSRC, "internal.h"), os.path.join(REPO_DIR, "include", "suika_reshard.h")]
+SOURCES = [os.path.join(CSRC, f) for f in ("plan.cpp", "act.cpp", "exec.cu", "optim.cu", "embed.cu", "logprob.cu")]
+DEPS = SOURCES + [os.path.join(CSRC, "internal.h"), os.path.join(CSRC, "train.cuh"), os.path.join(REPO_DIR, "include", "suika_reshard.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
