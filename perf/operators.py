@@ -232,7 +232,7 @@ def _clip(case, s):
     if own:
         from suika_b200.optimizer import clip_grads, grad_sumsq
         norm = clip_grads(s["grads"], case["max_norm"], sumsq=grad_sumsq(s["grads"]).add_(s["others"]))
-        return {"norm": norm, "grad": s["grad"]}
+        return {"norm": norm.reshape(1), "grad": s["grad"]}
     g = s["grad"]
     norm = (g.float().square().sum(dtype=torch.float64) + s["others"]).sqrt().float()
     c = (case["max_norm"] / (norm + 1e-6)).clamp(max=1.0)
