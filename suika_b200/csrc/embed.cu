@@ -7,7 +7,7 @@
 // order. Tokens are sorted by row (stable), so that a row's tokens are neighbours, and every sum is
 // taken in 32 bits in an order that depends on the ids alone: no float atomics, the same bits on
 // every run. Three launches: (1) one cluster sorts in distributed shared memory while every other
-// CTA clears the output, (2) tiles of sorted tokens are summed, (3) rows longer than a tile are
+// CTA clears the output, (2) tiles of 16 sorted tokens are summed, (3) rows longer than a tile are
 // joined from their pieces. The bound is HBM: grad_out read once, the gradient written once.
 #include "train.cuh"
 
@@ -41,7 +41,8 @@ __global__ void __launch_bounds__(256) lookup_kernel(const void* ids, bool wide,
   const int64_t units = n * segs;
   const int vecs = hidden / E;
   using P = Pack<T, E>;
-  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (int64_t)gridDim.x * 8) {
+  const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (u < units) {
     const int64_t i = u / segs;
     const int v0 = (int)(u - i * segs) * 128 + lane;
     const int64_t r = load_id(ids, wide, i) - lo;
@@ -68,6 +69,7 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortMaxItems = 8;      // per thread
 constexpr int kSortMaxCluster = 8;    // the portable cluster size
 constexpr int64_t kSortMax = (int64_t)kSortThreads * kSortMaxItems * kSortMaxCluster;  // 65536 tokens
+constexpr int kBins = 512;
 constexpr uint32_t kPadKey = 0xffffffffu;
 
 struct SortArgs {
@@ -77,22 +79,29 @@ struct SortArgs {
   int64_t lo;
   int64_t rows;
   int bits;        // of the largest key, `rows` (a token the shard does not hold)
+  int digit;       // bits a pass, at most 9
   uint32_t* keys;  // sorted rows
   int32_t* toks;   // their tokens
+  int32_t* long_rows;  // a count for the sums, cleared here
   char* fill;      // output to clear, or null
   uint64_t fill_bytes;
 };
 
-__device__ void clear_range(char* p, uint64_t bytes, uint64_t cta, uint64_t ctas) {
+// A clearing CTA writes one run of 64 KB.
+constexpr int kClearBytes = 64 * 1024;
+__device__ void clear_run(char* p, uint64_t bytes, uint64_t cta) {
   const uint64_t head = min(bytes, (uint64_t)((16 - ((uintptr_t)p & 15)) & 15));
   const uint64_t vecs = (bytes - head) / 16, tail = bytes - head - vecs * 16;
   if (cta == 0 && threadIdx.x < head) p[threadIdx.x] = 0;
   if (cta == 0 && threadIdx.x < tail) p[head + vecs * 16 + threadIdx.x] = 0;
   char* body = p + head;
-  for (uint64_t i = cta * kSortThreads + threadIdx.x; i < vecs; i += ctas * kSortThreads) st16(body + i * 16, make_uint4(0, 0, 0, 0));
+  const uint64_t v0 = cta * (kClearBytes / 16) + threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < kClearBytes / 16 / kSortThreads; ++u)
+    if (v0 + u * kSortThreads < vecs) st16(body + (v0 + u * kSortThreads) * 16, make_uint4(0, 0, 0, 0));
 }
 
-// Stable radix sort, 8 bits a pass, by one cluster. CTA c holds positions [c * CAP, (c + 1) * CAP) of the
+// Stable radix sort by one cluster, up to 9 bits a pass (18 bits, 262143 rows, are two passes). CTA c holds positions [c * CAP, (c + 1) * CAP) of the
 // array as (key, token) pairs in its shared memory; per pass a warp ranks its items among equal
 // digits (match_any), counts are summed over warps, CTAs (through distributed shared memory) and
 // digits, and every item is stored where it belongs, in whichever CTA that is. Items sit in
@@ -105,16 +114,17 @@ __global__ void __launch_bounds__(kSortThreads) sort_fill_kernel(SortArgs a) {
   static_assert(CAP == 1 << SHIFT, "capacity is a power of two");
   extern __shared__ uint4 smem[];
   uint2* buf = reinterpret_cast<uint2*>(smem);                    // CAP pairs
-  uint16_t(*cnt)[256] = reinterpret_cast<uint16_t(*)[256]>(buf + CAP);  // per warp and digit, at most 32 * R
-  __shared__ uint32_t total[256], base[256], scan[8];
+  uint16_t(*cnt)[kBins] = reinterpret_cast<uint16_t(*)[kBins]>(buf + CAP);  // per warp and digit, at most 32 * R
+  __shared__ uint32_t total[kBins], base[kBins], scan[kBins / 32];
   cg::cluster_group cluster = cg::this_cluster();
   const int cs = cluster.num_blocks();
   if (blockIdx.x >= cs) {  // not in the sorting cluster
-    clear_range(a.fill, a.fill_bytes, blockIdx.x - cs, gridDim.x - cs);
+    clear_run(a.fill, a.fill_bytes, blockIdx.x - cs);
     return;
   }
   const int me = cluster.block_rank(), w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t below = (1u << lane) - 1;
+  if (me == 0 && threadIdx.x == 0) *a.long_rows = 0;
   uint2 item[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -126,17 +136,18 @@ __global__ void __launch_bounds__(kSortThreads) sort_fill_kernel(SortArgs a) {
     }
     item[r] = make_uint2(key, (uint32_t)i);
   }
-  for (int shift = 0; shift < a.bits; shift += 8) {
+  const uint32_t mask = (1u << a.digit) - 1;
+  for (int shift = 0; shift < a.bits; shift += a.digit) {
     if (shift) {
 #pragma unroll
       for (int r = 0; r < R; ++r) item[r] = buf[w * 32 * R + r * 32 + lane];
     }
-    for (int i = threadIdx.x; i < 32 * 128; i += kSortThreads) reinterpret_cast<uint32_t*>(cnt)[i] = 0;
+    for (int i = threadIdx.x; i < 32 * kBins / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(cnt)[i] = 0;
     __syncthreads();
     uint32_t rank[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint32_t d = (item[r].x >> shift) & 255;
+      const uint32_t d = (item[r].x >> shift) & mask;
       const uint32_t peers = __match_any_sync(~0u, d);
       const uint32_t before = cnt[w][d];
       __syncwarp();
@@ -145,7 +156,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_fill_kernel(SortArgs a) {
       __syncwarp();
     }
     __syncthreads();
-    if (threadIdx.x < 256) {
+    if (threadIdx.x < kBins) {
       uint32_t sum = 0;
 #pragma unroll 8
       for (int k = 0; k < 32; ++k) {
@@ -157,7 +168,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_fill_kernel(SortArgs a) {
     }
     cluster.sync();
     uint32_t all = 0, before = 0, excl = 0;
-    if (threadIdx.x < 256) {
+    if (threadIdx.x < kBins) {
       for (int c = 0; c < cs; ++c) {
         const uint32_t t = cluster.map_shared_rank(total, c)[threadIdx.x];
         if (c < me) before += t;
@@ -173,14 +184,14 @@ __global__ void __launch_bounds__(kSortThreads) sort_fill_kernel(SortArgs a) {
       if (lane == 31) scan[w] = incl;
     }
     __syncthreads();
-    if (threadIdx.x < 256) {
+    if (threadIdx.x < kBins) {
       for (int k = 0; k < w; ++k) excl += scan[k];
       base[threadIdx.x] = excl + before;
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint32_t d = (item[r].x >> shift) & 255;
+      const uint32_t d = (item[r].x >> shift) & mask;
       const uint32_t to = base[d] + cnt[w][d] + rank[r];
       cluster.map_shared_rank(buf, to >> SHIFT)[to & (CAP - 1)] = item[r];
     }
@@ -197,123 +208,137 @@ __global__ void __launch_bounds__(kSortThreads) sort_fill_kernel(SortArgs a) {
 
 // ---- sums ---------------------------------------------------------------------------------
 
-constexpr int kMaxTile = 64;  // sorted tokens per CTA
-constexpr int kCols = 8;      // columns per thread
+constexpr int kTile = 16;  // sorted tokens per tile
+constexpr int kCols = 8;   // columns per lane
+constexpr int kSpan = 32 * kCols;
+constexpr int kBatch = 4;  // tokens whose vectors a lane has in flight
 
 struct SumArgs {
   const uint32_t* keys;
   const int32_t* toks;
   int32_t n;
-  int32_t tile;
   int64_t rows;
   int32_t hidden;
+  int32_t spans;  // of kSpan columns
   int64_t grad_stride;
   float scale;
-  bool accumulate;
-  float* partial;  // [tiles][2][hidden]: the piece of a long row that enters a tile, and the one that leaves it
+  float* partial;     // [tiles][2][hidden]: the piece of a long row that enters a tile, and the one that leaves it
+  int32_t* long_rows; // [0]: how many; then the tiles where a long row starts
 };
 
-// First position in [lo, hi) whose key is not below `key` (upper: above it).
-__device__ __forceinline__ int bound_of(const uint32_t* keys, int lo, int hi, uint32_t key, bool upper) {
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (upper ? keys[mid] <= key : keys[mid] < key) lo = mid + 1; else hi = mid;
-  }
-  return lo;
-}
-
 template <class G, int E>
-__device__ __forceinline__ void add_out(G* out, int64_t at, const float* x, bool accumulate) {
-  Pack<G, E>* p = reinterpret_cast<Pack<G, E>*>(out + at);
+__device__ __forceinline__ void store_out(G* out, int64_t at, const float* x) {
   Pack<G, E> v;
-  if (accumulate) v = *p;
 #pragma unroll
-  for (int e = 0; e < E; ++e) v.x[e] = from_f32<G>(accumulate ? to_f32<G>(v.x[e]) + x[e] : x[e]);
-  *p = v;
+  for (int e = 0; e < E; ++e) v.x[e] = from_f32<G>(x[e]);
+  *reinterpret_cast<Pack<G, E>*>(out + at) = v;
 }
 
-// A CTA sums the rows that start among its `tile` sorted tokens, for blockDim.x * 8 columns. A row of
-// at most `tile` tokens is summed whole by the CTA where it starts (reading at most tile - 1 tokens of the next
-// tile); a longer one is cut at the tiles' borders and its pieces go to `partial` for the join. So
-// no CTA sums more than 2 * tile - 1 tokens, however uneven the ids are. Four tokens' vectors are
-// loaded before the first is added: with 16-bit gradients that is 64 bytes in flight per thread.
-template <class T, class G, int E>
-__global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* out) {
+// A warp sums the rows that start among the 16 sorted tokens of its tile, for 256 columns. A row of at most 16
+// tokens is summed whole by the tile where it starts (up to 15 tokens of the next tile are read); a
+// longer one is cut at the tiles' borders, and its pieces go to `partial` for the join. So no warp sums more than
+// 31 tokens, however uneven the ids are. The keys from one tile before to one after are held
+// two to a lane; where rows start is one 64-bit mask. The vectors of four tokens (and, when adding to a
+// gradient, the rows that they end) are loaded before the first is added; warps need no barrier.
+template <class T, class G, int E, bool ACC>
+__global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* out, int64_t units) {
   constexpr int NV = kCols / E;
-  __shared__ uint32_t keys[3 * kMaxTile];
-  __shared__ int32_t toks[2 * kMaxTile];
-  const int s = blockIdx.x * a.tile, e = min(s + a.tile, a.n);
-  const int w0 = max(s - a.tile, 0), w1 = min(e + a.tile, a.n);
-  for (int i = w0 + threadIdx.x; i < w1; i += blockDim.x) keys[i - w0] = a.keys[i];
-  for (int i = s + threadIdx.x; i < w1; i += blockDim.x) toks[i - s] = a.toks[i];
-  __syncthreads();
-  // the range [pos, end) of positions this CTA sums
-  int pos = s, end = e;
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= units) return;
+  const int lane = threadIdx.x & 31;
+  const int tile = (int)(unit / a.spans);
+  const int col0 = (int)(unit - (int64_t)tile * a.spans) * kSpan + lane * E;
+  // window position j is sorted position w0 + j; the tile is [16, 32)
+  const int w0 = tile * kTile - kTile;
+  auto key_at = [&](int j) { return w0 + j < 0 ? kPadKey - 1 : w0 + j < a.n && j < 3 * kTile ? a.keys[w0 + j] : kPadKey; };
+  const uint32_t k0 = key_at(lane), k1 = key_at(lane + 32);
+  const int t1 = w0 + lane + 32 < a.n && lane < kTile ? a.toks[w0 + lane + 32] : 0;
+  const int t0 = lane >= kTile && w0 + lane < a.n ? a.toks[w0 + lane] : 0;
+  const uint32_t p0 = __shfl_up_sync(~0u, k0, 1), q1 = __shfl_up_sync(~0u, k1, 1), last0 = __shfl_sync(~0u, k0, 31);
+  const uint64_t starts = (uint64_t)__ballot_sync(~0u, lane > 0 && k0 != p0) | (uint64_t)__ballot_sync(~0u, k1 != (lane ? q1 : last0)) << 32;
+  const uint64_t held = (uint64_t)__ballot_sync(~0u, k0 < a.rows) | (uint64_t)__ballot_sync(~0u, k1 < a.rows) << 32;
+  auto start_after = [&](int j) { const uint64_t m = starts >> (j + 1); return m ? j + __ffsll(m) : 48; };  // j < 47
+  int pos = kTile, end = 2 * kTile;
   bool head = false, tail = false;
-  if (s > 0 && keys[s - 1 - w0] == keys[s - w0]) {  // a row that started earlier
-    const uint32_t k = keys[s - w0];
-    const int a0 = w0 + bound_of(keys, 0, s - w0, k, false), b0 = w0 + bound_of(keys, s - w0, w1 - w0, k, true);
-    // where the window cuts the row off, it is longer than a tile
-    const bool is_long = (a0 == w0 && w0 > 0) || b0 - a0 > a.tile;
-    if (is_long) head = true; else pos = min(b0, e);
+  if (!(starts >> kTile & 1)) {  // a row that started earlier
+    const uint64_t m = starts & ((1ull << kTile) - 1);
+    const int b = start_after(kTile);
+    // without a start in the window it reaches back more than a tile
+    if (m == 0 || b - (63 - __clzll(m)) > kTile) head = true; else pos = min(b, end);
   }
-  if (pos < e) {
-    const uint32_t k = keys[e - 1 - w0];
-    const int a1 = w0 + bound_of(keys, pos - w0, e - w0, k, false), b1 = w0 + bound_of(keys, e - 1 - w0, w1 - w0, k, true);
-    if (!(head && a1 == s)) {  // the last row starts in this tile
-      if (b1 - a1 > a.tile) tail = true; else end = b1;
+  if (pos >= end) return;
+  {
+    const uint64_t m = starts & 0xffffffffull & ~((1ull << pos) - 1);
+    if (m) {  // the last row starts in this tile
+      const int b = start_after(31);
+      if (b - (63 - __clzll(m)) > kTile) tail = true; else end = b;
+    }
+  }
+  {  // tokens that the shard does not hold are sorted last
+    const uint64_t m = ~held >> pos;
+    const int stop = m ? pos + __ffsll(m) - 1 : end;
+    if (stop < end) {
+      end = stop;
+      tail = false;
     }
   }
   if (pos >= end) return;
-  const int col0 = (int)blockIdx.y * blockDim.x * kCols + threadIdx.x * E;
-  const int step = blockDim.x * E;
+  const uint32_t head_key = __shfl_sync(~0u, k0, kTile);
+  if (tail && lane == 0 && col0 == 0) a.long_rows[1 + atomicAdd(a.long_rows, 1)] = tile;  // their order does not matter
   bool on[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v) on[v] = col0 + v * step < a.hidden;
+  for (int v = 0; v < NV; ++v) on[v] = col0 + v * 32 * E < a.hidden;
   float acc[NV][E];
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
-    for (int q = 0; q < E; ++q) acc[v][q] = 0.f;
-  constexpr int U = 4;
-  for (int p = pos; p < end; p += U) {
-    Pack<T, E> x[U][NV];
+    for (int c = 0; c < E; ++c) acc[v][c] = 0.f;
+  for (int p = pos; p < end; p += kBatch) {
+    Pack<T, E> x[kBatch][NV];
+    Pack<G, E> old[kBatch][NV];
+    uint32_t row[kBatch];
+    bool last[kBatch], piece[kBatch];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (p + u < end && keys[p + u - w0] < a.rows) {
-        const T* g = grad + (int64_t)toks[p + u - s] * a.grad_stride + col0;
+    for (int u = 0; u < kBatch; ++u) {
+      const int q = p + u;
+      const int64_t t = q < 32 ? __shfl_sync(~0u, t0, q & 31) : __shfl_sync(~0u, t1, q & 31);
+      row[u] = q < 32 ? __shfl_sync(~0u, k0, q & 31) : __shfl_sync(~0u, k1, q & 31);
+      last[u] = q + 1 >= end || (starts >> ((q + 1) & 63) & 1);
+      piece[u] = (head && row[u] == head_key) || (tail && q + 1 == end);
+      if (q < end) {
+        const T* g = grad + t * a.grad_stride + col0;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-          if (on[v]) x[u][v] = *reinterpret_cast<const Pack<T, E>*>(g + v * step);
+          if (on[v]) x[u][v] = *reinterpret_cast<const Pack<T, E>*>(g + v * 32 * E);
+        if (ACC && last[u] && !piece[u]) {
+          const G* o = out + (int64_t)row[u] * a.hidden + col0;
+#pragma unroll
+          for (int v = 0; v < NV; ++v)
+            if (on[v]) old[u][v] = *reinterpret_cast<const Pack<G, E>*>(o + v * 32 * E);
+        }
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int q = p + u;
-      if (q >= end) break;
-      const uint32_t row = keys[q - w0];
-      if (row >= a.rows) return;  // tokens that this shard does not hold, sorted last
+    for (int u = 0; u < kBatch; ++u) {
+      if (p + u >= end) break;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
         if (on[v]) {
 #pragma unroll
           for (int c = 0; c < E; ++c) acc[v][c] += to_f32<T>(x[u][v].x[c]);
         }
-      const bool last = q + 1 == end || keys[q + 1 - w0] != row;
-      if (!last) continue;
-      const bool is_head = head && row == keys[s - w0], is_tail = tail && q + 1 == end && !is_head;
+      if (!last[u]) continue;
+      const bool leaves = !(head && row[u] == head_key);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         if (on[v]) {
-          const int col = col0 + v * step;
-          if (is_head || is_tail) {
-            float* to = a.partial + ((int64_t)blockIdx.x * 2 + (is_tail ? 1 : 0)) * a.hidden + col;
-#pragma unroll
-            for (int c = 0; c < E; ++c) to[c] = acc[v][c];
+          const int col = col0 + v * 32 * E;
+          if (piece[u]) {
+            store_out<float, E>(a.partial, ((int64_t)tile * 2 + leaves) * a.hidden + col, acc[v]);
           } else {
 #pragma unroll
-            for (int c = 0; c < E; ++c) acc[v][c] *= a.scale;
-            add_out<G, E>(out, (int64_t)row * a.hidden + col, acc[v], a.accumulate);
+            for (int c = 0; c < E; ++c) acc[v][c] = ACC ? fmaf(acc[v][c], a.scale, to_f32<G>(old[u][v].x[c])) : acc[v][c] * a.scale;
+            store_out<G, E>(out, (int64_t)row[u] * a.hidden + col, acc[v]);
           }
         }
 #pragma unroll
@@ -323,37 +348,41 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* o
   }
 }
 
-// Joins the pieces of a row longer than a tile: the CTA of the tile where the row starts adds the piece
-// that leaves this tile and those that enter the next ones, in order.
+// Joins the pieces of the rows longer than a tile: the piece that leaves the tile where the row starts and
+// those that enter the next ones. A CTA takes 32 columns of a row; its 8 warps each add an equal run of
+// consecutive pieces in order, and the runs are added in order: the same bits always.
 template <class G>
-__global__ void __launch_bounds__(256) join_kernel(SumArgs a, G* out) {
-  const int s = blockIdx.x * a.tile, e = s + a.tile;
-  if (e >= a.n) return;
-  const uint32_t k = a.keys[e - 1];
-  if (k >= a.rows || a.keys[e] != k || (s > 0 && a.keys[s - 1] == k)) return;
-  const int a0 = bound_of(a.keys, s, e, k, false);
-  if (a0 + a.tile >= a.n || a.keys[a0 + a.tile] != k) return;  // at most a tile long: summed whole already
-  int pieces = 0;  // tiles after this one that the row enters
-  for (int t = blockIdx.x + 1;; t += blockDim.x) {
-    const int64_t at = (int64_t)(t + (int)threadIdx.x) * a.tile;
-    const int got = __syncthreads_count(at < a.n && a.keys[at] == k);
-    pieces += got;
-    if (got < (int)blockDim.x) break;
-  }
-  for (int col = blockIdx.y * blockDim.x + threadIdx.x; col < a.hidden; col += gridDim.y * blockDim.x) {
-    const float* p = a.partial + (int64_t)blockIdx.x * 2 * a.hidden + col;
-    float acc = p[a.hidden];
-    int t = 1;
-    for (; t + 7 <= pieces; t += 8) {
-      float x[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = p[(int64_t)(t + u) * 2 * a.hidden];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) acc += x[u];
+__global__ void __launch_bounds__(256) join_kernel(SumArgs a, G* out, bool accumulate) {
+  __shared__ float sums[8][32];
+  const int chunks = (a.hidden + 31) / 32, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t units = (int64_t)a.long_rows[0] * chunks;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int tile = a.long_rows[1 + unit / chunks], col = (int)(unit % chunks) * 32 + lane;
+    const uint32_t k = a.keys[tile * kTile + kTile - 1];
+    int pieces = 1;  // one leaves this tile, one enters each of the next as long as the row goes on
+    for (int t = tile + 1;; t += blockDim.x) {
+      const int64_t at = (int64_t)(t + (int)threadIdx.x) * kTile;
+      const int got = __syncthreads_count(at < a.n && a.keys[at] == k);
+      pieces += got;
+      if (got < (int)blockDim.x) break;
     }
-    for (; t <= pieces; ++t) acc += p[(int64_t)t * 2 * a.hidden];
-    acc *= a.scale;
-    add_out<G, 1>(out, (int64_t)k * a.hidden + col, &acc, a.accumulate);
+    const int i0 = (int)((int64_t)pieces * w / 8), i1 = (int)((int64_t)pieces * (w + 1) / 8);
+    float acc = 0.f;
+    if (col < a.hidden) {
+      const float* p = a.partial + (int64_t)tile * 2 * a.hidden + col;  // piece i of the row: [tile + i][i == 0]
+#pragma unroll 8
+      for (int i = i0; i < i1; ++i) acc += p[((int64_t)i * 2 + (i == 0)) * a.hidden];
+    }
+    sums[w][lane] = acc;
+    __syncthreads();
+    if (w == 0 && col < a.hidden) {
+      float total = sums[0][lane];
+#pragma unroll
+      for (int q = 1; q < 8; ++q) total += sums[q][lane];
+      G* to = out + (int64_t)k * a.hidden + col;
+      *to = from_f32<G>(accumulate ? fmaf(total, a.scale, to_f32<G>(*to)) : total * a.scale);
+    }
+    __syncthreads();
   }
 }
 
@@ -369,12 +398,13 @@ int vector_elements(int most, uint64_t a, uint64_t a_stride_bytes, int a_bytes, 
 }
 
 template <class T>
-int launch_lookup(const rs_embed_opts& o, const void* ids, const void* weight, void* out, int sms, cudaStream_t st) {
+int launch_lookup(const rs_embed_opts& o, const void* ids, const void* weight, void* out, cudaStream_t st) {
   const int b = sizeof(T);
   const int e = vector_elements(16 / b, (uint64_t)weight, (uint64_t)o.weight_stride * b, b, (uint64_t)out, (uint64_t)o.hidden * b, b, (int)o.hidden);
   const int segs = (int)((o.hidden / e + 127) / 128);
   const int64_t units = o.n_tokens * segs;
-  const int grid = (int)std::min<int64_t>((units + 7) / 8, (int64_t)sms * 16);
+  if ((units + 7) / 8 > 0x7fffffff) return tfail(RS_ERR_CAPACITY, "rs_embed_lookup: too many tokens and columns in one call");
+  const unsigned grid = (unsigned)((units + 7) / 8);
   auto go = [&](auto E) {
     constexpr int EE = decltype(E)::value;
     lookup_kernel<T, EE><<<grid, 256, 0, st>>>(ids, o.wide_ids != 0, o.n_tokens, (const T*)weight, o.weight_stride, o.rows, (int)o.hidden, o.lo,
@@ -399,33 +429,28 @@ int check_opts(const char* what, const rs_embed_opts* o) {
 }
 
 struct GradPlan {
-  int cluster = 1, items = 1, tile = 8, tiles = 0, threads = 32, chunks = 1;
-  uint64_t keys = 0, toks = 0, partial = 0, bytes = 0;
+  int cluster = 1, items = 1, tiles = 0;
+  uint64_t keys = 0, toks = 0, partial = 0, long_rows = 0, bytes = 0;
 };
 
-// The cluster grows before the items per thread do (eight CTAs sort 8192 tokens one per thread). A tile
-// holds as many tokens as still leave about six CTAs to an SM, 8 to 64: short tiles keep the sums of a
-// few tokens parallel, long ones cost fewer pieces.
-GradPlan plan_grad(const rs_embed_opts& o, int sms) {
+// The cluster grows before the items per thread do (eight CTAs sort 8192 tokens one per thread).
+GradPlan plan_grad(const rs_embed_opts& o) {
   GradPlan p;
   const int64_t n = o.n_tokens;
   while (p.cluster < kSortMaxCluster && (int64_t)p.cluster * kSortThreads < n) p.cluster *= 2;
   while ((int64_t)p.cluster * kSortThreads * p.items < n) p.items *= 2;
-  const int64_t threads = (o.hidden + kCols - 1) / kCols;
-  p.threads = (int)std::min<int64_t>(256, std::max<int64_t>(32, (threads + 31) / 32 * 32));
-  p.chunks = (int)std::max<int64_t>(1, (o.hidden + (int64_t)p.threads * kCols - 1) / ((int64_t)p.threads * kCols));
-  while (p.tile < kMaxTile && n * p.chunks / p.tile > (int64_t)sms * 6) p.tile *= 2;
-  p.tiles = (int)((n + p.tile - 1) / p.tile);
+  p.tiles = (int)((n + kTile - 1) / kTile);
   auto slot = [&](uint64_t b) { const uint64_t at = p.bytes; p.bytes += (b + 255) / 256 * 256; return at; };
   p.keys = slot((uint64_t)n * 4);
   p.toks = slot((uint64_t)n * 4);
+  p.long_rows = slot((uint64_t)(p.tiles + 1) * 4);
   p.partial = slot(p.tiles > 1 ? (uint64_t)p.tiles * 2 * o.hidden * 4 : 0);
   return p;
 }
 
 template <int R>
 int launch_sort(const SortArgs& a, int cluster, int grid, cudaStream_t st) {
-  const size_t smem = (size_t)R * kSortThreads * sizeof(uint2) + 32 * 256 * sizeof(uint16_t);
+  const size_t smem = (size_t)R * kSortThreads * sizeof(uint2) + 32 * kBins * sizeof(uint16_t);
   if (smem > 40 * 1024) {  // with the static arrays, past the 48 KB that need no opt-in
     cudaError_t e = cudaFuncSetAttribute(sort_fill_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return tcuda(e, "rs_embed_grad: cudaFuncSetAttribute");
@@ -445,29 +470,35 @@ int launch_sort(const SortArgs& a, int cluster, int grid, cudaStream_t st) {
 }
 
 template <class T, class G>
-int launch_sums(const SumArgs& a, const GradPlan& p, const void* grad, void* out, cudaStream_t st) {
-  const int e = vector_elements(16 / (int)sizeof(T), (uint64_t)grad, (uint64_t)a.grad_stride * sizeof(T), sizeof(T),
-                                (uint64_t)out, (uint64_t)a.hidden * sizeof(G), sizeof(G), a.hidden);
-  const dim3 grid(p.tiles, p.chunks);
+int launch_sums(const SumArgs& a, const GradPlan& p, const void* grad, void* out, bool accumulate, int sms, cudaStream_t st) {
+  const int e = vector_elements(16 / (int)sizeof(T), (uint64_t)grad, (uint64_t)a.grad_stride * sizeof(T), sizeof(T), (uint64_t)out,
+                                (uint64_t)a.hidden * sizeof(G), sizeof(G), a.hidden);
+  const int64_t units = (int64_t)p.tiles * a.spans;
+  if ((units + 7) / 8 > 0x7fffffff) return tfail(RS_ERR_CAPACITY, "rs_embed_grad: too many tokens and columns in one call");
+  const unsigned grid = (unsigned)((units + 7) / 8);
   auto go = [&](auto E) {
     constexpr int EE = decltype(E)::value;
-    sum_kernel<T, G, EE><<<grid, p.threads, 0, st>>>(a, (const T*)grad, (G*)out);
+    if (accumulate) sum_kernel<T, G, EE, true><<<grid, 256, 0, st>>>(a, (const T*)grad, (G*)out, units);
+    else sum_kernel<T, G, EE, false><<<grid, 256, 0, st>>>(a, (const T*)grad, (G*)out, units);
   };
   if (e == 8) { if constexpr (sizeof(T) == 2) go(std::integral_constant<int, 8>{}); }
   else if (e == 4) go(std::integral_constant<int, 4>{});
   else if (e == 2) go(std::integral_constant<int, 2>{});
   else go(std::integral_constant<int, 1>{});
   int rc = tcuda(cudaGetLastError(), "rs_embed_grad: launch (sums)");
-  if (rc != RS_OK || p.tiles < 2) return rc;
-  join_kernel<G><<<dim3(p.tiles, (a.hidden + 255) / 256), 256, 0, st>>>(a, (G*)out);
+  if (rc != RS_OK || p.tiles < 2) return rc;  // one tile has no row longer than a tile
+  // a row longer than a tile starts in every other tile at most
+  const int64_t most = (int64_t)p.tiles * ((a.hidden + 31) / 32);
+  join_kernel<G><<<(unsigned)std::min<int64_t>(most, (int64_t)sms * 8), 256, 0, st>>>(a, (G*)out, accumulate);
   return tcuda(cudaGetLastError(), "rs_embed_grad: launch (join)");
 }
 
 template <class T>
-int sums_of(const SumArgs& a, const GradPlan& p, uint32_t grad_dtype, const void* grad, void* out, cudaStream_t st) {
-  if (grad_dtype == RS_F32) return launch_sums<T, float>(a, p, grad, out, st);
-  if (grad_dtype == RS_BF16) return launch_sums<T, __nv_bfloat16>(a, p, grad, out, st);
-  return launch_sums<T, __half>(a, p, grad, out, st);
+int sums_of(const SumArgs& a, const GradPlan& p, const rs_embed_opts& o, const void* grad, void* out, int sms, cudaStream_t st) {
+  const bool acc = o.accumulate != 0;
+  if (o.grad_dtype == RS_F32) return launch_sums<T, float>(a, p, grad, out, acc, sms, st);
+  if (o.grad_dtype == RS_BF16) return launch_sums<T, __nv_bfloat16>(a, p, grad, out, acc, sms, st);
+  return launch_sums<T, __half>(a, p, grad, out, acc, sms, st);
 }
 
 }  // namespace
@@ -486,11 +517,10 @@ int rs_embed_lookup(const rs_embed_opts* opts, const void* ids_dev, const void* 
       return tfail(RS_ERR_ARG, "rs_embed_lookup: an address is not aligned to its elements");
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_embed_lookup: cudaSetDevice");
-    const int sms = sm_count(device);
     cudaStream_t st = (cudaStream_t)stream;
-    if (o.dtype == RS_F32) return launch_lookup<float>(o, ids_dev, weight_dev, out_dev, sms, st);
-    if (o.dtype == RS_BF16) return launch_lookup<__nv_bfloat16>(o, ids_dev, weight_dev, out_dev, sms, st);
-    return launch_lookup<__half>(o, ids_dev, weight_dev, out_dev, sms, st);
+    if (o.dtype == RS_F32) return launch_lookup<float>(o, ids_dev, weight_dev, out_dev, st);
+    if (o.dtype == RS_BF16) return launch_lookup<__nv_bfloat16>(o, ids_dev, weight_dev, out_dev, st);
+    return launch_lookup<__half>(o, ids_dev, weight_dev, out_dev, st);
   });
 }
 
@@ -499,7 +529,7 @@ int rs_embed_grad_workspace_bytes(const rs_embed_opts* opts, int32_t device, uin
   if (rc != RS_OK) return rc;
   if (!bytes) return tfail(RS_ERR_ARG, "rs_embed_grad_workspace_bytes: NULL result");
   if (opts->n_tokens > kSortMax) return tfail(RS_ERR_CAPACITY, "rs_embed_grad: more than 65536 tokens in one call");
-  *bytes = std::max<uint64_t>(256, plan_grad(*opts, sm_count(device)).bytes);
+  *bytes = std::max<uint64_t>(256, plan_grad(*opts).bytes);
   return RS_OK;
 }
 
@@ -522,7 +552,7 @@ int rs_embed_grad(const rs_embed_opts* opts, const void* ids_dev, const void* gr
       return o.accumulate ? RS_OK : tcuda(cudaMemsetAsync(grad_dev, 0, out_bytes, st), "rs_embed_grad: cudaMemsetAsync");
     if (!ids_dev || !grad_out_dev || (uint64_t)ids_dev % (o.wide_ids ? 8 : 4) || (uint64_t)grad_out_dev % b)
       return tfail(RS_ERR_ARG, "rs_embed_grad: NULL or misaligned ids or output gradient");
-    const GradPlan p = plan_grad(o, sms);
+    const GradPlan p = plan_grad(o);
     if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 256)
       return tfail(RS_ERR_CAPACITY, "rs_embed_grad: workspace too small or not 256-byte aligned");
     char* ws = (char*)workspace;
@@ -533,15 +563,18 @@ int rs_embed_grad(const rs_embed_opts* opts, const void* ids_dev, const void* gr
     s.lo = o.lo;
     s.rows = o.rows;
     while (s.bits < 32 && (uint64_t)o.rows >> s.bits) ++s.bits;
+    const int passes = (s.bits + 8) / 9;
+    s.digit = (s.bits + passes - 1) / passes;
     s.keys = (uint32_t*)(ws + p.keys);
     s.toks = (int32_t*)(ws + p.toks);
+    s.long_rows = (int32_t*)(ws + p.long_rows);
     int grid = p.cluster;
     if (!o.accumulate) {
       s.fill = (char*)grad_dev;
       s.fill_bytes = out_bytes;
-      // one clearing CTA per SM, fewer where there is little to clear (64 KB each)
-      const int64_t ctas = std::min<int64_t>(sms, (int64_t)((out_bytes + 65535) / 65536));
-      grid += (int)((ctas + p.cluster - 1) / p.cluster * p.cluster);
+      const uint64_t runs = (out_bytes + kClearBytes - 1) / kClearBytes;
+      if (runs > 0x7fffff00) return tfail(RS_ERR_CAPACITY, "rs_embed_grad: gradient too large");
+      grid += (int)((runs + p.cluster - 1) / p.cluster * p.cluster);
     }
     rc = p.items == 1 ? launch_sort<1>(s, p.cluster, grid, st) : p.items == 2 ? launch_sort<2>(s, p.cluster, grid, st)
        : p.items == 4 ? launch_sort<4>(s, p.cluster, grid, st) : launch_sort<8>(s, p.cluster, grid, st);
@@ -550,16 +583,16 @@ int rs_embed_grad(const rs_embed_opts* opts, const void* ids_dev, const void* gr
     a.keys = s.keys;
     a.toks = s.toks;
     a.n = s.n;
-    a.tile = p.tile;
     a.rows = o.rows;
     a.hidden = (int32_t)o.hidden;
+    a.spans = (int32_t)((o.hidden + kSpan - 1) / kSpan);
     a.grad_stride = o.grad_stride;
     a.scale = o.scale;
-    a.accumulate = o.accumulate != 0;
     a.partial = (float*)(ws + p.partial);
-    if (o.dtype == RS_F32) return sums_of<float>(a, p, o.grad_dtype, grad_out_dev, grad_dev, st);
-    if (o.dtype == RS_BF16) return sums_of<__nv_bfloat16>(a, p, o.grad_dtype, grad_out_dev, grad_dev, st);
-    return sums_of<__half>(a, p, o.grad_dtype, grad_out_dev, grad_dev, st);
+    a.long_rows = s.long_rows;
+    if (o.dtype == RS_F32) return sums_of<float>(a, p, o, grad_out_dev, grad_dev, sms, st);
+    if (o.dtype == RS_BF16) return sums_of<__nv_bfloat16>(a, p, o, grad_out_dev, grad_dev, sms, st);
+    return sums_of<__half>(a, p, o, grad_out_dev, grad_dev, sms, st);
   });
 }
 

@@ -147,17 +147,28 @@ __device__ __forceinline__ Stat warp_join(Stat st) {
   return st;
 }
 
+// One 64-bit number per logit whose order is that of the alternatives: larger logit first (-0 as 0), then
+// lower index.
+__device__ __forceinline__ uint64_t rank_key(float v, int i) {
+  uint32_t b = __float_as_uint(v + 0.f);
+  b ^= b >> 31 ? 0xffffffffu : 0x80000000u;
+  return (uint64_t)b << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  uint32_t b = (uint32_t)(k >> 32);
+  return __uint_as_float(b ^ (b >> 31 ? 0x80000000u : 0xffffffffu));
+}
+constexpr uint64_t kNoKey = 0;  // below every logit's (that of -inf is 0x007fffff << 32 and more)
+__device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k; }
+
 // The k first of `count` candidates in shared memory, by counting how many come before each.
-__device__ __forceinline__ void place_candidates(const float* val, const int* idx, int count, int k, float* out_val, int* out_idx) {
+__device__ __forceinline__ void place_candidates(const uint64_t* cand, int count, int k, uint64_t* best) {
   for (int c = threadIdx.x; c < count; c += kThreads) {
-    const float v = val[c];
-    const int i = idx[c];
+    const uint64_t mine = cand[c];
     int r = 0;
-    for (int d = 0; d < count; ++d) r += before(val[d], idx[d], v, i);
-    if (r < k) {
-      out_val[r] = v;
-      out_idx[r] = i;
-    }
+#pragma unroll 8
+    for (int d = 0; d < count; ++d) r += cand[d] > mine;
+    if (r < k) best[r] = mine;
   }
 }
 
@@ -169,10 +180,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(FwdArgs a) {
   extern __shared__ float notes[];  // [kNotes][kThreads] where alternatives are asked for
   __shared__ Stat warp_stat[8];
   __shared__ float lane_max[8][32];
-  __shared__ float cand_val[kMaxCand];
-  __shared__ int cand_idx[kMaxCand];
-  __shared__ float best_val[kMaxTop];
-  __shared__ int best_idx[kMaxTop];
+  __shared__ uint64_t cand[kMaxCand];
+  __shared__ uint64_t best[kMaxTop];
   __shared__ Stat cta_stat;
   __shared__ float bound;
   __shared__ int n_cand;
@@ -255,19 +264,13 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(FwdArgs a) {
     }
   }
   if (k) {
-    if (tid < kMaxTop) {
-      best_val[tid] = -INFINITY;
-      best_idx[tid] = INT_MAX;
-    }
+    if (tid < kMaxTop) best[tid] = kNoKey;
     __syncthreads();
     const float least = bound;
     auto offer = [&](float f, int i) {
       if (f >= least) {
         const int at = atomicAdd(&n_cand, 1);  // their order does not matter: they are ranked by value and index
-        if (at < kMaxCand) {
-          cand_val[at] = f;
-          cand_idx[at] = i;
-        }
+        if (at < kMaxCand) cand[at] = rank_key(f, i);
       }
     };
     for (int s = 0, v = v0 + tid; v < v1; ++s) {
@@ -289,21 +292,17 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(FwdArgs a) {
     __syncthreads();
     const int count = n_cand;
     if (count <= kMaxCand) {
-      place_candidates(cand_val, cand_idx, count, k, best_val, best_idx);
+      place_candidates(cand, count, k, best);
       __syncthreads();
     } else {
       // Too many logits as large as the bound (a nearly constant or mostly masked row): k searches
       // for the first logit after the last one chosen.
-      float pv = INFINITY;
-      int pi = -1;
+      uint64_t chosen = ~0ull;
       for (int r = 0; r < k; ++r) {
-        float bv = -INFINITY;
-        int bi = INT_MAX;
+        uint64_t next = kNoKey;
         auto look = [&](float f, int i) {
-          if (before(pv, pi, f, i) && before(f, i, bv, bi)) {
-            bv = f;
-            bi = i;
-          }
+          const uint64_t key = rank_key(f, i);
+          if (!isnan(f) && key < chosen && key > next) next = key;
         };
         for (int v = v0 + tid; v < v1; v += kThreads) {
           float f[N];
@@ -314,32 +313,16 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(FwdArgs a) {
         if (tid < loose) look(to_f32<T>(z[loose_at]), loose_at);
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
-          const float ov = __shfl_xor_sync(~0u, bv, o);
-          const int oi = __shfl_xor_sync(~0u, bi, o);
-          if (before(ov, oi, bv, bi)) {
-            bv = ov;
-            bi = oi;
-          }
+          const uint64_t other = __shfl_xor_sync(~0u, next, o);
+          if (other > next) next = other;
         }
-        __syncthreads();  // the last round's read of cand_* is over
-        if (lane == 0) {
-          cand_val[w] = bv;
-          cand_idx[w] = bi;
-        }
+        __syncthreads();  // the last round's reads of cand are over
+        if (lane == 0) cand[w] = next;
         __syncthreads();
-        bv = cand_val[0];
-        bi = cand_idx[0];
-        for (int q = 1; q < 8; ++q)
-          if (before(cand_val[q], cand_idx[q], bv, bi)) {
-            bv = cand_val[q];
-            bi = cand_idx[q];
-          }
-        if (tid == 0) {
-          best_val[r] = bv;
-          best_idx[r] = bi;
-        }
-        pv = bv;
-        pi = bi;
+        for (int q = 0; q < 8; ++q)
+          if (cand[q] > next) next = cand[q];
+        if (tid == 0) best[r] = next;
+        chosen = next;
       }
       __syncthreads();
     }
@@ -356,17 +339,12 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(FwdArgs a) {
       if (k) {
         for (int i = tid; i < cs * k; i += kThreads) {
           const int c = i / k, r = i - c * k;
-          cand_val[i] = cluster.map_shared_rank(best_val, c)[r];
-          cand_idx[i] = cluster.map_shared_rank(best_idx, c)[r];
+          cand[i] = cluster.map_shared_rank(best, c)[r];
         }
         __syncthreads();
-        // entries that no logit filled stand at (-inf, INT_MAX) and take no place
-        if (tid < kMaxTop) {
-          best_val[tid] = -INFINITY;
-          best_idx[tid] = INT_MAX;
-        }
+        if (tid < kMaxTop) best[tid] = kNoKey;
         __syncthreads();
-        place_candidates(cand_val, cand_idx, cs * k, k, best_val, best_idx);
+        place_candidates(cand, cs * k, k, best);
       }
     }
     cluster.sync();  // the others' shared memory is read until here
@@ -390,15 +368,16 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(FwdArgs a) {
     }
   }
   if (tid < k) {
-    const float v = best_val[tid];
-    const int i = best_idx[tid];
+    const bool none = best[tid] == kNoKey;
+    const float v = none ? -INFINITY : key_value(best[tid]);
+    const int i = none ? -1 : key_index(best[tid]);
     if (a.record) {
       float* r = a.record + row * (4 + 2 * k) + 4;
       r[tid] = v;
-      r[k + tid] = __int_as_float(i == INT_MAX ? -1 : i);
+      r[k + tid] = __int_as_float(i);
     } else {
       a.top_value[row * k + tid] = log_prob_of(v, t);
-      a.top_index[row * k + tid] = i == INT_MAX ? -1 : a.lo + i;
+      a.top_index[row * k + tid] = none ? -1 : a.lo + i;
     }
   }
 }

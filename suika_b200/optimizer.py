@@ -79,63 +79,66 @@ def counted_spans(layout, rank: int) -> Counted:
     return out
 
 
-def _check_grads(tensors: List[torch.Tensor], what: str) -> torch.device:
-    """One CUDA device, contiguous, a type the kernels take."""
-    dev = tensors[0].device
-    if dev.type != "cuda":
+def _refuse(t: torch.Tensor, index: int, what: str) -> None:
+    """Raise for a tensor that the kernels do not take."""
+    if t.device.type != "cuda":
         raise ValueError(f"{what} must be CUDA tensors")
-    index = dev.index
-    for i in map(torch.Tensor.get_device, tensors):
-        if i != index:
-            raise ValueError(f"{what} must share one device")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
+    if t.get_device() != index:
+        raise ValueError(f"{what} must share one device")
+    if not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
-    return dev
-
-
-def _codes(tensors: Iterable[torch.Tensor], what: str) -> List[int]:
-    try:
-        return [DTYPE_CODES[t.dtype] for t in tensors]
-    except KeyError as e:
-        raise ValueError(f"{what} of {e.args[0]}: float32, bfloat16 and float16 are taken") from None
+    raise ValueError(f"{what} of {t.dtype}: float32, bfloat16 and float16 are taken")
 
 
 def _named(grads: Grads) -> Tuple[Optional[List[str]], List[torch.Tensor]]:
     """(names or None, tensors); entries of None (a parameter without a gradient) are left out."""
     if hasattr(grads, "items"):
         kept = [(n, g) for n, g in grads.items() if g is not None]
-        return [n for n, _ in kept], [g for _, g in kept]
-    return None, [g for g in grads if g is not None]
+        names, tensors = [n for n, _ in kept], [g for _, g in kept]
+    else:
+        names, tensors = None, [g for g in grads if g is not None]
+    if not tensors:
+        raise ValueError("no gradients")
+    if tensors[0].device.type != "cuda":
+        raise ValueError("gradients must be CUDA tensors")
+    return names, tensors
 
 
-def _span_table(names: Optional[List[str]], tensors: List[torch.Tensor], counted: Optional[Counted]) -> np.ndarray:
-    codes = _codes(tensors, "gradients")
-    if counted is None:
-        table = np.zeros(len(tensors), dtype=L.GRAD_SPAN_DTYPE)
-        table["grad_dev"] = list(map(torch.Tensor.data_ptr, tensors))
-        table["numel"] = list(map(torch.Tensor.numel, tensors))
-        table["dtype"] = codes
-        return table
+def _spans(tensors: List[torch.Tensor], what: str = "gradients"):
+    """(rs_grad_span array, its length) of whole tensors: one device, contiguous, a type the kernels take.
+    (A span is three 64-bit words, the type in the low half of the last.)"""
+    index = tensors[0].get_device()
+    words: List[int] = []
+    for t in tensors:
+        code = DTYPE_CODES.get(t.dtype)
+        if code is None or t.get_device() != index or not t.is_contiguous():
+            _refuse(t, index, what)
+        words += (t.data_ptr(), t.numel(), code)
+    return (C.c_uint64 * len(words))(*words), len(tensors)
+
+
+def _counted_spans(names: Optional[List[str]], tensors: List[torch.Tensor], counted: Counted):
     if names is None:
         raise ValueError("counted spans go by name: give the gradients as {name: tensor}")
-    rows = []
-    for name, t, code in zip(names, tensors, codes):
+    _spans(tensors)  # the checks
+    words: List[int] = []
+    for name, t in zip(names, tensors):
         if name not in counted:
             raise AssertionError(f"no counted spans for {name}")
         for off, n in counted[name]:
             if off < 0 or n < 0 or off + n > t.numel():
                 raise AssertionError(f"{name}: counted span [{off}, {off + n}) leaves a gradient of {t.numel()} elements")
-            rows.append((t.data_ptr() + off * t.element_size(), n, code, 0))
-    return np.array(rows, dtype=L.GRAD_SPAN_DTYPE) if rows else np.zeros(0, dtype=L.GRAD_SPAN_DTYPE)
+            words += (t.data_ptr() + off * t.element_size(), n, DTYPE_CODES[t.dtype])
+    return (C.c_uint64 * len(words))(*words), len(words) // 3
 
 
-def _sumsq(table: np.ndarray, dev: torch.device) -> torch.Tensor:
+def _sumsq(spans, n: int, dev: torch.device) -> torch.Tensor:
     lib = L.load()
     nb = C.c_uint64()
-    L.check(lib.rs_grad_sumsq_workspace_bytes(len(table), C.byref(nb)))
+    L.check(lib.rs_grad_sumsq_workspace_bytes(n, C.byref(nb)))
     workspace = torch.empty(nb.value, dtype=torch.uint8, device=dev)
     out = torch.empty(1, dtype=torch.float64, device=dev)
-    L.check(lib.rs_grad_sumsq(table.ctypes.data, len(table), workspace.data_ptr(), nb.value, out.data_ptr(), dev.index, raw_stream(dev.index)))
+    L.check(lib.rs_grad_sumsq(spans, n, workspace.data_ptr(), nb.value, out.data_ptr(), dev.index, raw_stream(dev.index)))
     return out
 
 
@@ -144,10 +147,8 @@ def grad_sumsq(grads: Grads, counted: Optional[Counted] = None) -> torch.Tensor:
     float64 tensor of one element on their device, summed in 64 bits. `counted` (counted_spans):
     only what this rank counts; then an all-reduce over the ranks gives the global sum."""
     names, tensors = _named(grads)
-    if not tensors:
-        raise ValueError("no gradients")
-    dev = _check_grads(tensors, "gradients")
-    return _sumsq(_span_table(names, tensors, counted), dev)
+    spans, n = _spans(tensors) if counted is None else _counted_spans(names, tensors, counted)
+    return _sumsq(spans, n, tensors[0].device)
 
 
 def _check_sumsq(sumsq: torch.Tensor, dev: torch.device) -> None:
@@ -160,30 +161,21 @@ def clip_grads(grads: Grads, max_norm: float, *, sumsq: Optional[torch.Tensor] =
     """Scale the gradients in place by min(1, max_norm / (norm + 1e-6)) and return the norm (float32, on
     the device; nothing is synchronised). The norm is that of grad_sumsq(grads, counted), summed over
     `group` if one is given, or sqrt(sumsq) if the caller has the global sum of squares already. All
-    of every gradient is scaled, whether counted here or by another rank. A norm that is not finite
-    reaches the gradients, as in torch.nn.utils.clip_grad_norm_."""
+    of every gradient is scaled, whether counted here or by another rank; gradients that share memory
+    are refused. A norm that is not finite reaches the gradients, as in torch.nn.utils.clip_grad_norm_."""
     if not max_norm > 0:
         raise ValueError("max_norm must be positive")
     names, tensors = _named(grads)
-    if not tensors:
-        raise ValueError("no gradients")
-    dev = _check_grads(tensors, "gradients")
-    table = _span_table(None, tensors, None)
-    if len(table) > 1:  # a shared element would be scaled twice, or race
-        nonempty = table[table["numel"] > 0]
-        begin = nonempty["grad_dev"]
-        order = np.argsort(begin)
-        end = begin + nonempty["numel"] * np.where(nonempty["dtype"] == L.RS_F32, 4, 2).astype(np.uint64)
-        if (end[order][:-1] > begin[order][1:]).any():
-            raise ValueError("gradients share memory")
+    dev = tensors[0].device
+    spans, n = _spans(tensors)
     if sumsq is None:
-        sumsq = _sumsq(table if counted is None else _span_table(names, tensors, counted), dev)
+        sumsq = _sumsq(*((spans, n) if counted is None else _counted_spans(names, tensors, counted)), dev)
         if group is not None:
             dist.all_reduce(sumsq, group=group)
     else:
         _check_sumsq(sumsq, dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    L.check(L.load().rs_grad_clip(table.ctypes.data, len(table), sumsq.data_ptr(), max_norm, norm.data_ptr(), dev.index, raw_stream(dev.index)))
+    L.check(L.load().rs_grad_clip(spans, n, sumsq.data_ptr(), max_norm, norm.data_ptr(), dev.index, raw_stream(dev.index)))
     return norm
 
 
@@ -230,8 +222,11 @@ class ShardAdamW:
                     raise AssertionError(f"expected sub-fields mismatch: {name} has no {s}")
             p, m, v, w = ent["param"], ent["exp_avg"], ent["exp_avg_sq"], ent.get("master")
             body = [t for t in (p, m, v, w) if t is not None]
-            if _check_grads(body, f"{name}'s sub-fields") != self.device:
-                raise ValueError("the state's tensors must share one device")
+            if self.device is None or self.device.type != "cuda":
+                raise ValueError(f"{name}'s sub-fields must be CUDA tensors")
+            for t in body:
+                if t.device != self.device or not t.is_contiguous() or t.dtype not in DTYPE_CODES:
+                    _refuse(t, self.device.index, f"{name}'s sub-fields")
             if any(t.shape != p.shape for t in body):
                 raise AssertionError(f"{name}'s sub-fields differ in shape")
             if m.dtype != v.dtype or m.dtype not in (torch.float32, torch.bfloat16):
@@ -243,8 +238,8 @@ class ShardAdamW:
                 raise AssertionError(f"{name}: a step of {step.numel()} elements")
             if step.dtype != torch.float32 or step.device != self.device:
                 step = ent["step"] = step.to(device=self.device, dtype=torch.float32)
-            code = _codes((p, m), f"{name}'s sub-fields")
-            table[i] = (0, p.data_ptr(), 0 if w is None else w.data_ptr(), m.data_ptr(), v.data_ptr(), step.data_ptr(), p.numel(), 0, 0, *code)
+            table[i] = (0, p.data_ptr(), 0 if w is None else w.data_ptr(), m.data_ptr(), v.data_ptr(), step.data_ptr(), p.numel(), 0, 0,
+                        DTYPE_CODES[p.dtype], DTYPE_CODES[m.dtype])
             self._shapes.append(p.shape)
             if name in no_decay:
                 self._decays[i] = 0
@@ -267,44 +262,47 @@ class ShardAdamW:
         """One update from {name: gradient}; names without a gradient (missing or None) stay as they are.
         Returns the norm before clipping (float32, on the device), or None without max_norm. `sumsq`:
         the global sum of squares, if the caller has it already."""
-        names, shapes, table = self.names, self._shapes, self._table
+        names, shapes, table, decays = self.names, self._shapes, self._table, self._decays
         gs = [grads.get(n) for n in names]
-        given = [g is not None for g in gs]
-        decays = self._decays
-        if not all(given):
-            gs = [g for g in gs if g is not None]
-            if not gs:
+        if any(g is None for g in gs):
+            given = [g is not None for g in gs]
+            if not any(given):
                 raise ValueError("no gradients")
-            names = [n for n, k in zip(names, given) if k]
-            shapes = [s for s, k in zip(shapes, given) if k]
+            names, gs, shapes = ([x for x, k in zip(xs, given) if k] for xs in (names, gs, shapes))
             table, decays = table[given], decays[given]
         if len(grads) > len(gs):
             extra = [n for n, g in grads.items() if g is not None and n not in self.state]
             if extra:
                 raise AssertionError(f"gradients of names that the state does not hold: {extra[:3]}")
-        if _check_grads(gs, "gradients") != self.device:
-            raise ValueError("gradients must be on the state's device")
-        if [g.shape for g in gs] != shapes:
-            bad = next(n for n, g, s in zip(names, gs, shapes) if g.shape != s)
-            raise AssertionError(f"{bad}: a gradient of another shape")
-        lib, dev = L.load(), self.device
-        stream = raw_stream(dev.index)
+        dev = self.device
+        index = dev.index
+        at: List[int] = []
+        codes: List[int] = []
+        for n, g, shape in zip(names, gs, shapes):
+            code = DTYPE_CODES.get(g.dtype)
+            if code is None or g.get_device() != index or not g.is_contiguous():
+                _refuse(g, index, "gradients")
+            if g.shape != shape:
+                raise AssertionError(f"{n}: a gradient of another shape")
+            at.append(g.data_ptr())
+            codes.append(code)
+        lib = L.load()
         norm = None
         if self.max_norm is not None:
             if sumsq is None:
-                sumsq = _sumsq(_span_table(names, gs, self.counted), dev)
+                sumsq = _sumsq(*(_spans(gs) if self.counted is None else _counted_spans(names, gs, self.counted)), dev)
                 if self.group is not None:
                     dist.all_reduce(sumsq, group=self.group)
             else:
                 _check_sumsq(sumsq, dev)
             norm = torch.empty((), dtype=torch.float32, device=dev)
-        table["grad_dev"] = list(map(torch.Tensor.data_ptr, gs))
-        table["grad_dtype"] = _codes(gs, "gradients")
+        table["grad_dev"] = at
+        table["grad_dtype"] = codes
         table["weight_decay"] = decays * np.float32(self.weight_decay)
         opts = L.RsAdamwOpts(self.lr, self.betas[0], self.betas[1], self.eps, self.max_norm or 0.0)
         nb = C.c_uint64()
         L.check(lib.rs_adamw_workspace_bytes(len(table), C.byref(nb)))
         workspace = torch.empty(nb.value, dtype=torch.uint8, device=dev)
-        L.check(lib.rs_adamw_step(table.ctypes.data, len(table), C.byref(opts), sumsq.data_ptr() if norm is not None else None,
-                                  norm.data_ptr() if norm is not None else None, workspace.data_ptr(), nb.value, dev.index, stream))
+        L.check(lib.rs_adamw_step(table.ctypes.data, len(table), C.byref(opts), None if norm is None else sumsq.data_ptr(),
+                                  None if norm is None else norm.data_ptr(), workspace.data_ptr(), nb.value, index, raw_stream(index)))
         return norm
