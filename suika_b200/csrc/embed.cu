@@ -223,7 +223,7 @@ struct SumArgs {
   int64_t grad_stride;
   float scale;
   float* partial;     // [tiles][2][hidden]: the piece of a long row that enters a tile, and the one that leaves it
-  int32_t* long_rows; // [0]: how many; then the tiles where a long row starts
+  int32_t* long_rows; // [0]: how many; then, from [2], (tile where a long row starts, its pieces)
 };
 
 template <class G, int E>
@@ -248,16 +248,16 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* o
   const int lane = threadIdx.x & 31;
   const int tile = (int)(unit / a.spans);
   const int col0 = (int)(unit - (int64_t)tile * a.spans) * kSpan + lane * E;
-  // window position j is sorted position w0 + j; the tile is [16, 32)
+  // window position j is sorted position w0 + j; the tile is [kTile, 2 kTile)
   const int w0 = tile * kTile - kTile;
   auto key_at = [&](int j) { return w0 + j < 0 ? kPadKey - 1 : w0 + j < a.n && j < 3 * kTile ? a.keys[w0 + j] : kPadKey; };
   const uint32_t k0 = key_at(lane), k1 = key_at(lane + 32);
-  const int t1 = w0 + lane + 32 < a.n && lane < kTile ? a.toks[w0 + lane + 32] : 0;
-  const int t0 = lane >= kTile && w0 + lane < a.n ? a.toks[w0 + lane] : 0;
+  auto tok_at = [&](int j) { return j >= kTile && j < 3 * kTile && w0 + j < a.n ? a.toks[w0 + j] : 0; };
+  const int t0 = tok_at(lane), t1 = tok_at(lane + 32);
   const uint32_t p0 = __shfl_up_sync(~0u, k0, 1), q1 = __shfl_up_sync(~0u, k1, 1), last0 = __shfl_sync(~0u, k0, 31);
   const uint64_t starts = (uint64_t)__ballot_sync(~0u, lane > 0 && k0 != p0) | (uint64_t)__ballot_sync(~0u, k1 != (lane ? q1 : last0)) << 32;
   const uint64_t held = (uint64_t)__ballot_sync(~0u, k0 < a.rows) | (uint64_t)__ballot_sync(~0u, k1 < a.rows) << 32;
-  auto start_after = [&](int j) { const uint64_t m = starts >> (j + 1); return m ? j + __ffsll(m) : 48; };  // j < 47
+  auto start_after = [&](int j) { const uint64_t m = starts >> (j + 1); return m ? j + __ffsll(m) : 3 * kTile; };
   int pos = kTile, end = 2 * kTile;
   bool head = false, tail = false;
   if (!(starts >> kTile & 1)) {  // a row that started earlier
@@ -268,9 +268,9 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* o
   }
   if (pos >= end) return;
   {
-    const uint64_t m = starts & 0xffffffffull & ~((1ull << pos) - 1);
+    const uint64_t m = starts & ((1ull << 2 * kTile) - 1) & ~((1ull << pos) - 1);
     if (m) {  // the last row starts in this tile
-      const int b = start_after(31);
+      const int b = start_after(2 * kTile - 1);
       if (b - (63 - __clzll(m)) > kTile) tail = true; else end = b;
     }
   }
@@ -284,7 +284,19 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* o
   }
   if (pos >= end) return;
   const uint32_t head_key = __shfl_sync(~0u, k0, kTile);
-  if (tail && lane == 0 && col0 == 0) a.long_rows[1 + atomicAdd(a.long_rows, 1)] = tile;  // their order does not matter
+  if (tail && col0 == lane * E) {  // one piece leaves this tile, one enters each of the next as long as the row goes on
+    const uint32_t k = __shfl_sync(~0u, k0, 2 * kTile - 1);
+    int pieces = 1, got;
+    do {
+      const int64_t at = (int64_t)(tile + pieces + lane) * kTile;
+      got = __popc(__ballot_sync(~0u, at < a.n && a.keys[at] == k));
+      pieces += got;
+    } while (got == 32);
+    if (lane == 0) {
+      const int slot = atomicAdd(a.long_rows, 1);  // the order of the list does not matter
+      reinterpret_cast<int2*>(a.long_rows)[1 + slot] = make_int2(tile, pieces);
+    }
+  }
   bool on[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) on[v] = col0 + v * 32 * E < a.hidden;
@@ -349,38 +361,41 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* o
 }
 
 // Joins the pieces of the rows longer than a tile: the piece that leaves the tile where the row starts and
-// those that enter the next ones. A CTA takes 32 columns of a row; its 8 warps each add an equal run of
-// consecutive pieces in order, and the runs are added in order: the same bits always.
-template <class G>
+// those that enter the next ones. A CTA takes 32 x V columns of a row; its 8 warps each add an equal run
+// of consecutive pieces in order, and the runs are added in order: the same bits always.
+template <class G, int V>
 __global__ void __launch_bounds__(256) join_kernel(SumArgs a, G* out, bool accumulate) {
-  __shared__ float sums[8][32];
-  const int chunks = (a.hidden + 31) / 32, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  using P = Pack<float, V>;
+  __shared__ P sums[8][32];
+  const int chunks = (a.hidden + 32 * V - 1) / (32 * V), lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t units = (int64_t)a.long_rows[0] * chunks;
   for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const int tile = a.long_rows[1 + unit / chunks], col = (int)(unit % chunks) * 32 + lane;
-    const uint32_t k = a.keys[tile * kTile + kTile - 1];
-    int pieces = 1;  // one leaves this tile, one enters each of the next as long as the row goes on
-    for (int t = tile + 1;; t += blockDim.x) {
-      const int64_t at = (int64_t)(t + (int)threadIdx.x) * kTile;
-      const int got = __syncthreads_count(at < a.n && a.keys[at] == k);
-      pieces += got;
-      if (got < (int)blockDim.x) break;
-    }
+    const int2 row = reinterpret_cast<const int2*>(a.long_rows)[1 + unit / chunks];
+    const int tile = row.x, pieces = row.y, col = (int)(unit % chunks) * 32 * V + lane * V;
     const int i0 = (int)((int64_t)pieces * w / 8), i1 = (int)((int64_t)pieces * (w + 1) / 8);
-    float acc = 0.f;
+    P acc{};
     if (col < a.hidden) {
       const float* p = a.partial + (int64_t)tile * 2 * a.hidden + col;  // piece i of the row: [tile + i][i == 0]
 #pragma unroll 8
-      for (int i = i0; i < i1; ++i) acc += p[((int64_t)i * 2 + (i == 0)) * a.hidden];
+      for (int i = i0; i < i1; ++i) {
+        const P x = *reinterpret_cast<const P*>(p + ((int64_t)i * 2 + (i == 0)) * a.hidden);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc.x[e] += x.x[e];
+      }
     }
     sums[w][lane] = acc;
     __syncthreads();
     if (w == 0 && col < a.hidden) {
-      float total = sums[0][lane];
-#pragma unroll
-      for (int q = 1; q < 8; ++q) total += sums[q][lane];
+      const uint32_t k = a.keys[tile * kTile + kTile - 1];
       G* to = out + (int64_t)k * a.hidden + col;
-      *to = from_f32<G>(accumulate ? fmaf(total, a.scale, to_f32<G>(*to)) : total * a.scale);
+#pragma unroll
+      for (int q = 1; q < 8; ++q) {
+        const P x = sums[q][lane];
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc.x[e] += x.x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) to[e] = from_f32<G>(accumulate ? fmaf(acc.x[e], a.scale, to_f32<G>(to[e])) : acc.x[e] * a.scale);
     }
     __syncthreads();
   }
@@ -443,7 +458,7 @@ GradPlan plan_grad(const rs_embed_opts& o) {
   auto slot = [&](uint64_t b) { const uint64_t at = p.bytes; p.bytes += (b + 255) / 256 * 256; return at; };
   p.keys = slot((uint64_t)n * 4);
   p.toks = slot((uint64_t)n * 4);
-  p.long_rows = slot((uint64_t)(p.tiles + 1) * 4);
+  p.long_rows = slot((uint64_t)(p.tiles + 1) * 8);
   p.partial = slot(p.tiles > 1 ? (uint64_t)p.tiles * 2 * o.hidden * 4 : 0);
   return p;
 }
@@ -487,9 +502,11 @@ int launch_sums(const SumArgs& a, const GradPlan& p, const void* grad, void* out
   else go(std::integral_constant<int, 1>{});
   int rc = tcuda(cudaGetLastError(), "rs_embed_grad: launch (sums)");
   if (rc != RS_OK || p.tiles < 2) return rc;  // one tile has no row longer than a tile
-  // a row longer than a tile starts in every other tile at most
-  const int64_t most = (int64_t)p.tiles * ((a.hidden + 31) / 32);
-  join_kernel<G><<<(unsigned)std::min<int64_t>(most, (int64_t)sms * 8), 256, 0, st>>>(a, (G*)out, accumulate);
+  const int v = a.hidden % 4 == 0 ? 4 : 1;  // columns per lane
+  const int64_t most = (int64_t)(p.tiles - 1) * ((a.hidden + 32 * v - 1) / (32 * v));
+  const unsigned ctas = (unsigned)std::min<int64_t>(most, (int64_t)sms * 8);
+  if (v == 4) join_kernel<G, 4><<<ctas, 256, 0, st>>>(a, (G*)out, accumulate);
+  else join_kernel<G, 1><<<ctas, 256, 0, st>>>(a, (G*)out, accumulate);
   return tcuda(cudaGetLastError(), "rs_embed_grad: launch (join)");
 }
 

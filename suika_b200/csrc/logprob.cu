@@ -6,8 +6,8 @@
 // log S - A / S. The differences z - m are taken first, so logits of any size (the type's lowest
 // value as a mask among them) neither overflow nor lose the digits that the exponent needs. The
 // top alternatives need no second pass over the row: each thread notes the maximum of every 64
-// bytes it reads, the k-th largest of the block's 32 lane maxima is a bound that at least k logits reach, and
-// only the noted places that reach it are read again. All sums are in 32 bits.
+// bytes it reads, the k-th largest maximum of 64 groups of threads is a bound that at least k logits reach (44 do for
+// k = 32, fewer for less), and only the noted places that reach it are read again. All sums are in 32 bits.
 //
 // HBM is the bound for many rows (each logit is read once, the gradient reads and writes once).
 // Few rows are split over the CTAs of a cluster, which join through distributed shared memory.
@@ -24,11 +24,12 @@ namespace {
 
 using namespace suika_train;
 
-constexpr int kThreads = 256;
-constexpr int kUnroll = 4;     // 16-byte vectors a thread has in flight
-constexpr int kMaxTop = 32;    // lane maxima that bound the k-th largest
+constexpr int kThreads = 256;  // of the gradient and the merge
+constexpr int kUnroll = 4;     // 16-byte vectors of a batch of loads, per thread
+constexpr int kMaxTop = 32;
 constexpr int kMaxCand = 1024; // logits kept for the exact choice
-constexpr int kNotes = 40;     // noted maxima per thread: 40 KB for 256 threads
+constexpr int kMaxHits = 512;  // noted places read again
+constexpr int kNotes = 16;     // noted maxima per thread: 16 KB for 256 threads, so that they do not cost resident CTAs
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_fast(float t) {
@@ -60,26 +61,106 @@ __device__ __forceinline__ Stat join(const Stat& x, const Stat& y) {
   return r;
 }
 
-// One more logit below or at the maximum.
-__device__ __forceinline__ void add_logit(Stat& st, float base, float z) {
-  const float t = (z - base) * kLog2e;
-  const float e = exp2_fast(t);
-  st.s += e;
-  st.a = fmaf(e, fmaxf(t, -1e4f), st.a);  // 0 * -inf would be NaN; e is 0 there
+// Two fp32 values in a register pair, for the packed add, multiply and fused multiply-add.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float x, float y) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 t) {
+  const float2 v = unpair(t);
+  return pair(exp2_fast(v.x), exp2_fast(v.y));
 }
 
-__device__ __forceinline__ void raise_max(Stat& st, float m) {
+// Vectors of 16-bit logits with -inf raised to a finite value whose exponential is 0 just the same (0 * -inf
+// would be NaN), two at a time; NaN stays. The value has to lie far below the row's base, and their
+// difference times log2(e) must not overflow: a base beyond moderate() takes the other path.
+template <class T> __device__ __forceinline__ uint4 raise_low(uint4 v) { return v; }
+template <> __device__ __forceinline__ uint4 raise_low<__nv_bfloat16>(uint4 v) {
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+  const __nv_bfloat162 low = __float2bfloat162_rn(-1e37f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], low);
+  return v;
+}
+template <> __device__ __forceinline__ uint4 raise_low<__half>(uint4 v) {
+  __half2* h = reinterpret_cast<__half2*>(&v);
+  const __half2 low = __float2half2_rn(-65504.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], low);
+  return v;
+}
+template <class T> __device__ __forceinline__ bool moderate(float) { return false; }
+template <> __device__ __forceinline__ bool moderate<__nv_bfloat16>(float base) { return fabsf(base) <= 1e36f; }
+template <> __device__ __forceinline__ bool moderate<__half>(float base) { return fabsf(base) <= 60000.f; }
+
+// A thread's running sums, two of each.
+struct Sums {
+  float m;
+  f32x2 s, a;
+};
+
+__device__ __forceinline__ void raise_max(Sums& st, float m) {
   if (m > st.m) {
-    const float t = fmaxf((base_of(st.m) - m) * kLog2e, -1e4f);
-    if (st.m == -INFINITY) {
-      // sums so far are 0, or NaN
-    } else {
-      const float c = exp2_fast(t);
-      st.a = c * (st.a + st.s * t);
-      st.s *= c;
+    if (st.m != -INFINITY) {  // before that the sums are 0, or NaN
+      const float t = fmaxf((st.m - m) * kLog2e, -1e4f), c = exp2_fast(t);
+      st.a = mul2(pair(c, c), fma2(st.s, pair(t, t), st.a));
+      st.s = mul2(pair(c, c), st.s);
     }
     st.m = m;
   }
+}
+
+// One vector of logits at or below the maximum: s += e, a += e t with t = (z - m) log2(e), e = 2^t. RAISED: the
+// vector went through raise_low, and no t has to be kept from -inf.
+template <class T, bool RAISED>
+__device__ __forceinline__ void add_vector(Sums& st, float base, uint4 v) {
+  constexpr int N = Vec16<T>::N;
+  const f32x2 minus = pair(-base, -base), scale = pair(kLog2e, kLog2e);
+  float f[N];
+  unpack16<T>(RAISED ? raise_low<T>(v) : v, f);
+#pragma unroll
+  for (int q = 0; q < N; q += 2) {
+    const f32x2 t = mul2(add2(pair(f[q], f[q + 1]), minus), scale);
+    const f32x2 e = exp2_pair(t);
+    st.s = add2(st.s, e);
+    if (RAISED) {
+      st.a = fma2(e, t, st.a);
+    } else {
+      const float2 u = unpair(t);
+      st.a = fma2(e, pair(fmaxf(u.x, -1e4f), fmaxf(u.y, -1e4f)), st.a);
+    }
+  }
+}
+__device__ __forceinline__ void add_logit(Sums& st, float z) {
+  const float t = (z - base_of(st.m)) * kLog2e, e = exp2_fast(t);
+  st.s = add2(st.s, pair(e, 0.f));
+  st.a = fma2(pair(e, 0.f), pair(fmaxf(t, -1e4f), 0.f), st.a);
+}
+__device__ __forceinline__ Stat total(const Sums& st) {
+  const float2 s = unpair(st.s), a = unpair(st.a);
+  return Stat{st.m, s.x + s.y, a.x + a.y};
 }
 
 // The order of the alternatives: larger logit first, then the lower index.
@@ -163,7 +244,7 @@ __device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k;
 
 // The k first of `count` candidates in shared memory, by counting how many come before each.
 __device__ __forceinline__ void place_candidates(const uint64_t* cand, int count, int k, uint64_t* best) {
-  for (int c = threadIdx.x; c < count; c += kThreads) {
+  for (int c = threadIdx.x; c < count; c += blockDim.x) {
     const uint64_t mine = cand[c];
     int r = 0;
 #pragma unroll 8
@@ -172,172 +253,263 @@ __device__ __forceinline__ void place_candidates(const uint64_t* cand, int count
   }
 }
 
-// A cluster of CTAs per row; CTA c takes the c-th share of the row's vectors. Logits before the first
-// 16-byte border of a row and after its last whole vector go to single threads of CTA 0.
+// A CTA's share of a row: whole 16-byte vectors [v0, v1) from `body`. The logits before the row's first 16-byte
+// border and after its last whole vector (at most 14) go to one thread each of the row's first CTA.
 template <class T>
-__global__ void __launch_bounds__(kThreads) forward_kernel(FwdArgs a) {
-  constexpr int N = Vec16<T>::N;
-  extern __shared__ float notes[];  // [kNotes][kThreads] where alternatives are asked for
-  __shared__ Stat warp_stat[8];
-  __shared__ float lane_max[8][32];
+struct Share {
+  const T* z;
+  const uint4* body;
+  int head, vecs, v0, v1, loose;
+  __device__ __forceinline__ Share(const FwdArgs& a, int64_t row, int part, int cs) {
+    constexpr int N = Vec16<T>::N;
+    const int cols = (int)a.cols;
+    z = reinterpret_cast<const T*>(a.logits) + row * a.stride;
+    head = min(cols, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T));
+    vecs = (cols - head) / N;
+    v0 = (int)((int64_t)vecs * part / cs);
+    v1 = (int)((int64_t)vecs * (part + 1) / cs);
+    body = reinterpret_cast<const uint4*>(z + head);
+    loose = part == 0 ? cols - vecs * N : 0;
+  }
+  __device__ __forceinline__ int loose_at(int t) const { return t < head ? t : t + vecs * Vec16<T>::N; }
+};
+
+// A cluster of cs CTAs per row. (Persistent CTAs that load the next row's first vectors while they finish one
+// need the registers of a third of the warps: 4096 rows of 152064 bf16 logits took 244 us instead of 206.)
+template <class T, int THREADS>
+__global__ void __launch_bounds__(THREADS) forward_kernel(FwdArgs a, int cs) {
+  constexpr int N = Vec16<T>::N, WARPS = THREADS / 32;
+  extern __shared__ float notes[];  // [kNotes][THREADS] where alternatives are asked for
+  __shared__ float warp_max[WARPS], lane_max[WARPS][32];
+  __shared__ float2 warp_sum[WARPS];
   __shared__ uint64_t cand[kMaxCand];
   __shared__ uint64_t best[kMaxTop];
   __shared__ Stat cta_stat;
   __shared__ float bound;
-  __shared__ int n_cand;
+  __shared__ float group_max[64];
+  __shared__ int n_cand, n_hits, step_sum[WARPS];
+  __shared__ int hits[kMaxHits];
   cg::cluster_group cluster = cg::this_cluster();
-  const int cs = cluster.num_blocks(), part = cluster.block_rank();
+  const int part = cs > 1 ? (int)cluster.block_rank() : 0;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, k = a.top;
   const int64_t row = blockIdx.x / cs;
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const T* z = reinterpret_cast<const T*>(a.logits) + row * a.stride;
-  const int cols = (int)a.cols;
-  const int head = min(cols, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T));
-  const int vecs = (cols - head) / N;
-  const int v0 = (int)((int64_t)vecs * part / cs), v1 = (int)((int64_t)vecs * (part + 1) / cs);
-  const uint4* body = reinterpret_cast<const uint4*>(z + head);
-  const int loose = part == 0 ? cols - vecs * N : 0;  // head and tail logits, one per thread (at most 14)
-  const int loose_at = tid < head ? tid : tid + vecs * N;
-  const int k = a.top;
+  const Share<T> sh(a, row, part, cs);
+  // the target's logit, read now and used at the end
+  float target = INFINITY;
+  if (tid == 0) {
+    const int64_t at = load_target(a.targets, a.wide, row) - a.lo;
+    if (at >= 0 && at < a.cols) target = to_f32<T>(sh.z[at]);
+  }
+  const float loose_z = tid < sh.loose ? to_f32<T>(sh.z[sh.loose_at(tid)]) : -INFINITY;
 
-  Stat st{-INFINITY, 0.f, 0.f};
-  float own_max = -INFINITY;  // of whole vectors, for the bound
+  Sums st{-INFINITY, 0, 0};
   int note = 0, in_note = 0;
   float noted = -INFINITY;
-  for (int v = v0 + tid; v < v1; v += kUnroll * kThreads) {
+  for (int v = sh.v0 + tid; v < sh.v1; v += kUnroll * THREADS) {
     uint4 x[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (v + u * THREADS < sh.v1) x[u] = ld16(sh.body + v + u * THREADS);
     float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (v + u * kThreads < v1) x[u] = ld16(body + v + u * kThreads);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (v + u * kThreads < v1) mx = fmaxf(mx, max_of<T>(x[u]));
+      if (v + u * THREADS < sh.v1) mx = fmaxf(mx, max_of<T>(x[u]));
     raise_max(st, mx);
     const float base = base_of(st.m);
+    if (sizeof(T) == 4 || moderate<T>(base)) {  // one branch per batch: one per vector cost a third of the rate
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (v + u * kThreads < v1) {
-        float f[N];
-        unpack16<T>(x[u], f);
+      for (int u = 0; u < kUnroll; ++u)
+        if (v + u * THREADS < sh.v1) add_vector<T, sizeof(T) == 2>(st, base, x[u]);
+    } else {
 #pragma unroll
-        for (int q = 0; q < N; ++q) add_logit(st, base, f[q]);
-      }
+      for (int u = 0; u < kUnroll; ++u)
+        if (v + u * THREADS < sh.v1) add_vector<T, false>(st, base, x[u]);
     }
     if (k) {
       noted = fmaxf(noted, mx);
       if (++in_note == a.per_note) {
-        notes[note * kThreads + tid] = noted;
+        notes[note * THREADS + tid] = noted;
         ++note;
         in_note = 0;
         noted = -INFINITY;
       }
     }
   }
-  if (k && in_note) notes[note * kThreads + tid] = noted;
-  if (tid < loose) {
-    const float f = to_f32<T>(z[loose_at]);
-    raise_max(st, f);
-    add_logit(st, base_of(st.m), f);
+  // every thread has a note for each of the CTA's batches, -inf past its last vector
+  const int batches = (sh.v1 - sh.v0 + kUnroll * THREADS - 1) / (kUnroll * THREADS);
+  const int notes_of_cta = (batches + a.per_note - 1) / a.per_note;
+  if (k && in_note) notes[note++ * THREADS + tid] = noted;
+  if (k && note < notes_of_cta) notes[note * THREADS + tid] = -INFINITY;
+  if (tid < sh.loose) {
+    raise_max(st, loose_z);
+    add_logit(st, loose_z);
   }
-  own_max = st.m;
-  const Stat ws = warp_join(st);
-  if (lane == 0) warp_stat[w] = ws;
-  if (k) lane_max[w][lane] = own_max;
-  if (tid == 0) n_cand = 0;
-  __syncthreads();
 
-  if (w == 0) {
-    Stat t = lane < 8 ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-    t = warp_join(t);
-    if (lane == 0) cta_stat = t;
-    if (k) {  // the k-th largest of 32 lane maxima: k logits at least are as large
-      float x = lane_max[0][lane];
+  // the CTA's maximum first, then sums that are already relative to it
+  float m = st.m;
 #pragma unroll
-      for (int r = 1; r < 8; ++r) x = fmaxf(x, lane_max[r][lane]);
-      int rank = 0;
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  if (lane == 0) warp_max[w] = m;
+  if (k) lane_max[w][lane] = st.m;
+  if (tid == 0) n_cand = n_hits = 0;
+  if (tid < kMaxTop) best[tid] = kNoKey;
+  __syncthreads();
+  m = warp_max[0];
 #pragma unroll
-      for (int o = 0; o < 32; ++o) {
-        const float y = __shfl_sync(~0u, x, o);
-        rank += before(y, o, x, lane);
-      }
-      if (rank == k - 1) bound = x;
+  for (int q = 1; q < WARPS; ++q) m = fmaxf(m, warp_max[q]);
+  {
+    raise_max(st, m);
+    Stat mine = total(st);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      mine.s += __shfl_xor_sync(~0u, mine.s, o);
+      mine.a += __shfl_xor_sync(~0u, mine.a, o);
     }
+    if (lane == 0) warp_sum[w] = make_float2(mine.s, mine.a);
   }
+  if (k && tid < 64) {  // threads t and t + 64 j form a group: its maximum
+    float y = -INFINITY;
+#pragma unroll
+    for (int r = tid >> 5; r < WARPS; r += 2) y = fmaxf(y, lane_max[r][lane]);
+    group_max[tid] = y;
+  }
+  __syncthreads();
+  Stat t{m, warp_sum[0].x, warp_sum[0].y};
+#pragma unroll
+  for (int q = 1; q < WARPS; ++q) {
+    t.s += warp_sum[q].x;
+    t.a += warp_sum[q].y;
+  }
+
   if (k) {
-    if (tid < kMaxTop) best[tid] = kNoKey;
+    if (tid < 64) {  // the k-th largest of the groups' maxima: k logits at least are as large
+      const float y = group_max[tid];
+      int rank = 0;
+#pragma unroll 16
+      for (int o = 0; o < 64; ++o) rank += before(group_max[o], o, y, tid);
+      if (rank == k - 1) bound = y;
+    }
     __syncthreads();
     const float least = bound;
-    auto offer = [&](float f, int i) {
-      if (f >= least) {
-        const int at = atomicAdd(&n_cand, 1);  // their order does not matter: they are ranked by value and index
-        if (at < kMaxCand) cand[at] = rank_key(f, i);
-      }
-    };
-    for (int s = 0, v = v0 + tid; v < v1; ++s) {
-      const bool look = notes[s * kThreads + tid] >= least;
-      for (int q = 0; q < a.per_note && v < v1; ++q, v += kUnroll * kThreads) {
-        if (!look) continue;
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          if (v + u * kThreads < v1) {
-            float f[N];
-            unpack16<T>(ld16(body + v + u * kThreads), f);
-#pragma unroll
-            for (int e = 0; e < N; ++e) offer(f[e], head + (v + u * kThreads) * N + e);
-          }
+    // Collects the logits from `least` on (strict: above it) from the noted places, one vector of them
+    // per thread: one latency for all. Their order does not matter, they are ranked by value and index.
+    auto collect = [&](bool strict) {
+      auto wanted = [&](float f) { return strict ? f > least : f >= least; };
+      auto offer = [&](float f, int i) {
+        if (wanted(f)) {
+          const int at = atomicAdd(&n_cand, 1);
+          if (at < kMaxCand) cand[at] = rank_key(f, i);
         }
-      }
-    }
-    if (tid < loose) offer(to_f32<T>(z[loose_at]), loose_at);
-    __syncthreads();
-    const int count = n_cand;
-    if (count <= kMaxCand) {
-      place_candidates(cand, count, k, best);
+      };
+      for (int s = 0; s < notes_of_cta; ++s)
+        if (wanted(notes[s * THREADS + tid])) {
+          const int at = atomicAdd(&n_hits, 1);
+          if (at < kMaxHits) hits[at] = s * THREADS + tid;
+        }
       __syncthreads();
-    } else {
-      // Too many logits as large as the bound (a nearly constant or mostly masked row): k searches
-      // for the first logit after the last one chosen.
-      uint64_t chosen = ~0ull;
-      for (int r = 0; r < k; ++r) {
-        uint64_t next = kNoKey;
-        auto look = [&](float f, int i) {
-          const uint64_t key = rank_key(f, i);
-          if (!isnan(f) && key < chosen && key > next) next = key;
-        };
-        for (int v = v0 + tid; v < v1; v += kThreads) {
+      const int found = min(n_hits, kMaxHits), per_hit = a.per_note * kUnroll;
+      for (int i = tid; i < found * per_hit; i += THREADS) {
+        const int hit = hits[i / per_hit], s = hit / THREADS;
+        const int v = sh.v0 + (hit - s * THREADS) + (s * per_hit + i % per_hit) * THREADS;
+        if (v < sh.v1) {
           float f[N];
-          unpack16<T>(ld16(body + v), f);
+          unpack16<T>(ld16(sh.body + v), f);
 #pragma unroll
-          for (int e = 0; e < N; ++e) look(f[e], head + v * N + e);
+          for (int e = 0; e < N; ++e) offer(f[e], sh.head + v * N + e);
         }
-        if (tid < loose) look(to_f32<T>(z[loose_at]), loose_at);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-          const uint64_t other = __shfl_xor_sync(~0u, next, o);
-          if (other > next) next = other;
-        }
-        __syncthreads();  // the last round's reads of cand are over
-        if (lane == 0) cand[w] = next;
-        __syncthreads();
-        for (int q = 0; q < 8; ++q)
-          if (cand[q] > next) next = cand[q];
-        if (tid == 0) best[r] = next;
-        chosen = next;
       }
+      if (tid < sh.loose) offer(loose_z, sh.loose_at(tid));
       __syncthreads();
+      return n_hits <= kMaxHits && n_cand <= kMaxCand;
+    };
+    if (collect(false)) {
+      place_candidates(cand, n_cand, k, best);
+    } else {
+      // Very many logits equal the bound (a masked or nearly constant row): those above it, then the first
+      // ones, in the order of the row, that equal it.
+      __syncthreads();
+      if (tid == 0) n_cand = n_hits = 0;
+      __syncthreads();
+      if (collect(true)) {
+        const int above = n_cand;
+        place_candidates(cand, above, k, best);
+        int placed = min(above, k);
+        // one step: each thread has up to N logits, in the order of the threads
+        auto step = [&](const float* f, int n, int at) {
+          int equal = 0;
+          for (int e = 0; e < n; ++e) equal += f[e] == least;
+          int before_me = equal;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(~0u, before_me, o);
+            if (lane >= o) before_me += y;
+          }
+          if (lane == 31) step_sum[w] = before_me;
+          __syncthreads();
+          int slot = placed + before_me - equal;
+          for (int q = 0; q < WARPS; ++q) {
+            if (q < w) slot += step_sum[q];
+            placed += step_sum[q];
+          }
+          for (int e = 0; e < n; ++e)
+            if (f[e] == least) {
+              if (slot < k) best[slot] = rank_key(f[e], at + e);
+              ++slot;
+            }
+          __syncthreads();
+        };
+        float f[N];
+        f[0] = loose_z;
+        if (part == 0 && placed < k) step(f, tid < min(sh.loose, sh.head) ? 1 : 0, tid);
+        for (int v = sh.v0; v < sh.v1 && placed < k; v += THREADS) {
+          const bool mine = v + tid < sh.v1;
+          if (mine) unpack16<T>(ld16(sh.body + v + tid), f);
+          step(f, mine ? N : 0, sh.head + (v + tid) * N);
+        }
+        f[0] = loose_z;
+        if (part == 0 && placed < k) step(f, tid >= sh.head && tid < sh.loose ? 1 : 0, sh.loose_at(tid));
+      } else {
+        // Large logits at a period that puts them all into a few groups: k searches for the first logit after
+        // the last one chosen.
+        uint64_t chosen = ~0ull;
+        for (int r = 0; r < k; ++r) {
+          uint64_t top = kNoKey;
+          auto look = [&](float f, int i) {
+            const uint64_t key = rank_key(f, i);
+            if (!isnan(f) && key < chosen && key > top) top = key;
+          };
+          for (int v = sh.v0 + tid; v < sh.v1; v += THREADS) {
+            float f[N];
+            unpack16<T>(ld16(sh.body + v), f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) look(f[e], sh.head + v * N + e);
+          }
+          if (tid < sh.loose) look(loose_z, sh.loose_at(tid));
+#pragma unroll
+          for (int o = 16; o; o >>= 1) {
+            const uint64_t other = __shfl_xor_sync(~0u, top, o);
+            if (other > top) top = other;
+          }
+          __syncthreads();  // the last round's reads of cand are over
+          if (lane == 0) cand[w] = top;
+          __syncthreads();
+          for (int q = 0; q < WARPS; ++q)
+            if (cand[q] > top) top = cand[q];
+          if (tid == 0) best[r] = top;
+          chosen = top;
+        }
+      }
     }
   }
 
   // join the CTAs of the row
   if (cs > 1) {
+    if (tid == 0) cta_stat = t;
     cluster.sync();
     if (part == 0) {
-      Stat t = cta_stat;
       for (int c = 1; c < cs; ++c) t = join(t, *cluster.map_shared_rank(&cta_stat, c));
-      __syncthreads();
-      if (tid == 0) cta_stat = t;
       if (k) {
-        for (int i = tid; i < cs * k; i += kThreads) {
+        for (int i = tid; i < cs * k; i += THREADS) {
           const int c = i / k, r = i - c * k;
           cand[i] = cluster.map_shared_rank(best, c)[r];
         }
@@ -349,14 +521,11 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(FwdArgs a) {
     }
     cluster.sync();  // the others' shared memory is read until here
     if (part != 0) return;
-  } else {
+  } else if (k) {
     __syncthreads();
   }
 
-  const Stat t = cta_stat;
   if (tid == 0) {
-    const int64_t at = a.targets ? load_target(a.targets, a.wide, row) - a.lo : -1;
-    const float target = at >= 0 && at < a.cols ? to_f32<T>(z[at]) : INFINITY;
     if (a.record) {
       float* r = a.record + row * (4 + 2 * k);
       r[0] = t.m;
@@ -443,7 +612,7 @@ struct BwdArgs {
   void* out;
   int64_t out_stride;
   int units;  // pieces of kUnroll * kThreads vectors in a row
-  int ctas;   // CTAs per row: one per piece, or one where the output is the logits (a row that is read again is then read before it is written)
+  int ctas;   // CTAs per row; one where the output is the logits (a row that is read again is then read before it is written)
 };
 
 // d z_j = g_lp (1[j = t] - p_j) - g_H p_j (log p_j + H) + g_lse p_j, p_j = e^(z_j - lse): one read and one
@@ -458,6 +627,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(BwdArgs a) {
   const int64_t target = load_target(a.targets, a.wide, row) - a.lo;
   const float lse = a.lse[row];
   const float h = a.entropy ? a.entropy[row] : 0.f, gh = a.grad_entropy ? a.grad_entropy[row] : 0.f;
+  const int target_col = target >= 0 && target < a.cols ? (int)target : -1;
   const bool ignored = a.sharded ? target + a.lo < 0 : target < 0 || target >= a.cols;
   const float gl = ignored ? 0.f : a.grad_logprob[row];
   const float gz = a.grad_lse ? a.grad_lse[row] : 0.f, gp = gl - gz;
@@ -472,13 +642,13 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(BwdArgs a) {
   // again, by each of its CTAs. (A shard alone cannot, and stays with lse.)
   float base = lse, rest = 0.f;
   if (!none && !a.sharded && fabsf(lse) > 1024.f && isfinite(lse)) {
-    Stat st{-INFINITY, 0.f, 0.f};
+    Sums far{-INFINITY, 0, 0};
     for (int j = threadIdx.x; j < cols; j += kThreads) {
       const float f = to_f32<T>(z[j]);
-      raise_max(st, f);
-      add_logit(st, base_of(st.m), f);
+      raise_max(far, f);
+      add_logit(far, f);
     }
-    st = warp_join(st);
+    Stat st = warp_join(total(far));
     __shared__ Stat part[8];
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = st;
     __syncthreads();  // every thread has read the row
@@ -487,32 +657,56 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(BwdArgs a) {
     base = st.m;
     rest = logf(st.s);
   }
-  auto one = [&](float f, int j) {
-    const float t = (f - base) - rest;
-    const float d = fmaxf(t, -1e4f);  // e is 0 below; -inf * 0 would be NaN
-    const float p = exp2_fast(t * kLog2e);
-    float g = -p * fmaf(gh, d + h, gp);
-    if (j == target) g += gl;
-    return none ? 0.f : g;
+  // with d = log p: gradient = p (wd d + w0), and g_lp more at the target
+  const float wd = -gh, w0 = -fmaf(gh, h, gp);
+  const bool raised = moderate<T>(base);
+  const f32x2 minus = pair(-base, -base), less = pair(-rest, -rest), scale = pair(kLog2e, kLog2e), wd2 = pair(wd, wd), w02 = pair(w0, w0);
+  auto two = [&](float x, float y) {
+    f32x2 d = add2(add2(pair(x, y), minus), less);
+    const f32x2 p = exp2_pair(mul2(d, scale));
+    if (!raised) {  // p is 0 below; -inf * 0 would be NaN
+      const float2 u = unpair(d);
+      d = pair(fmaxf(u.x, -1e4f), fmaxf(u.y, -1e4f));
+    }
+    return unpair(mul2(p, fma2(wd2, d, w02)));
   };
   const int per = kUnroll * kThreads;
   const uint4* src = reinterpret_cast<const uint4*>(z + head);
   uint4* dst = reinterpret_cast<uint4*>(out + head);
-  for (int unit = first; unit < a.units; unit += a.ctas) {
-    const int v = unit * per + threadIdx.x;
-    uint4 x[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (!none && v + u * kThreads < vecs) x[u] = ld16(src + v + u * kThreads);
+  // the next piece is loaded before this one is worked on
+  uint4 x[kUnroll];
+  auto load = [&](int unit) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int q = v + u * kThreads;
+      const int q = unit * per + threadIdx.x + u * kThreads;
+      if (!none && q < vecs) x[u] = ld16(src + q);
+    }
+  };
+  load(first);
+  for (int unit = first; unit < a.units; unit += a.ctas) {
+    uint4 now[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) now[u] = x[u];
+    load(unit + a.ctas);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int q = unit * per + threadIdx.x + u * kThreads;
       if (q >= vecs) break;
       float f[N];
       if (!none) {
-        unpack16<T>(x[u], f);
+        unpack16<T>(raised ? raise_low<T>(now[u]) : now[u], f);
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = one(f[e], head + q * N + e);
+        for (int e = 0; e < N; e += 2) {
+          const float2 g = two(f[e], f[e + 1]);
+          f[e] = g.x;
+          f[e + 1] = g.y;
+        }
+        const int at = target_col - (head + q * N);
+        if (at >= 0 && at < N) {
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (e == at) f[e] += gl;
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) f[e] = 0.f;
@@ -524,7 +718,9 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(BwdArgs a) {
   const int loose = cols - vecs * N;
   for (int i = first * kThreads + threadIdx.x; i < loose; i += a.ctas * kThreads) {
     const int j = i < head ? i : i + vecs * N;
-    out[j] = from_f32<T>(one(none ? 0.f : to_f32<T>(z[j]), j));
+    float f = none ? 0.f : to_f32<T>(z[j]);
+    if (raised) f = fmaxf(f, -1e37f) + (isnan(f) ? f : 0.f);
+    out[j] = from_f32<T>(none ? 0.f : two(f, 0.f).x + (j == target_col ? gl : 0.f));
   }
 }
 
@@ -542,25 +738,24 @@ int check_opts(const char* what, const rs_logprob_opts* o) {
   return RS_OK;
 }
 
-template <class T>
-int launch_forward(FwdArgs a, int sms, cudaStream_t st) {
+template <class T, int THREADS>
+int launch_forward_as(FwdArgs a, int cs, cudaStream_t st) {
   constexpr int N = Vec16<T>::N;
   const int64_t vecs = a.cols / N + 1;
-  // CTAs per row: few rows are split until two CTAs per SM are busy, while a share keeps two rounds of loads
-  int cs = 1;
-  while (cs < 8 && a.n * cs * 2 <= (int64_t)sms * 2 && vecs >= (int64_t)cs * 2 * kUnroll * kThreads) cs *= 2;
   size_t smem = 0;
   a.per_note = 1;
   if (a.top) {
-    const int64_t its = ((vecs + cs - 1) / cs + 1 + kUnroll * kThreads - 1) / (kUnroll * kThreads);
+    const int64_t its = ((vecs + cs - 1) / cs + 1 + kUnroll * THREADS - 1) / (kUnroll * THREADS);
     a.per_note = (int)((its + kNotes - 1) / kNotes);
-    smem = (size_t)((its + a.per_note - 1) / a.per_note) * kThreads * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(forward_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNotes * kThreads * (int)sizeof(float));
-    if (e != cudaSuccess) return tcuda(e, "rs_token_logprobs: cudaFuncSetAttribute");
+    smem = (size_t)((its + a.per_note - 1) / a.per_note) * THREADS * sizeof(float);
+    if (smem > 32 * 1024) {  // with the static arrays, past the 48 KB that need no opt-in
+      cudaError_t e = cudaFuncSetAttribute(forward_kernel<T, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return tcuda(e, "rs_token_logprobs: cudaFuncSetAttribute");
+    }
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.n * cs));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -569,7 +764,24 @@ int launch_forward(FwdArgs a, int sms, cudaStream_t st) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return tcuda(cudaLaunchKernelEx(&cfg, forward_kernel<T>, a), "rs_token_logprobs: launch");
+  return tcuda(cudaLaunchKernelEx(&cfg, forward_kernel<T, THREADS>, a, cs), "rs_token_logprobs: launch");
+}
+
+// Few rows are split over a cluster of up to 8 CTAs: until two CTAs per SM are busy, while a share keeps 960
+// vectors (15 KB; below that the join costs more than it saves), or, where shares stay above 64 KB, until five
+// are (300 rows of 152064 fp32 logits: 29 us, 42 in one CTA each). Shares of few rows take 512 threads (3
+// such rows: 10.2 us against 11.5 with 256), many short rows 128 (4096 rows of 1000: 12.2 us against 16.4), whose
+// other threads would idle.
+template <class T>
+int launch_forward(const FwdArgs& a, int sms, cudaStream_t st) {
+  const int64_t vecs = a.cols / Vec16<T>::N + 1;
+  int cs = 1;
+  while (cs < 8 && ((a.n * cs * 2 <= (int64_t)sms * 2 && vecs >= (int64_t)cs * 2 * 960) ||
+                    (a.n * cs * 2 <= (int64_t)sms * 5 && vecs >= (int64_t)cs * 2 * 4096)))
+    cs *= 2;
+  if (a.n * cs <= (int64_t)sms * 2 && vecs / cs >= 900) return launch_forward_as<T, 512>(a, cs, st);
+  if (vecs / cs <= 2048 && a.n > (int64_t)sms * 2) return launch_forward_as<T, 128>(a, cs, st);
+  return launch_forward_as<T, 256>(a, cs, st);
 }
 
 int forward(const char* what, const rs_logprob_opts* o, const void* logits, const void* targets, float* logprob, float* entropy, float* lse,
@@ -699,7 +911,9 @@ int rs_token_logprobs_grad(const rs_logprob_opts* opts, const void* logits_dev, 
       if (o.stride != grad_stride || o.n_rows == 1 || apart < width || apart + width > pitch)
         return tfail(RS_ERR_ARG, "rs_token_logprobs_grad: the gradient overlaps the logits without being them");
     }
-    a.ctas = same ? 1 : (int)units;
+    // up to four pieces per CTA, as long as sixteen CTAs per SM are left
+    const int64_t pieces = std::min<int64_t>(4, std::max<int64_t>(1, units * o.n_rows / ((int64_t)sm_count(device) * 16)));
+    a.ctas = same ? 1 : (int)((units + pieces - 1) / pieces);
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_token_logprobs_grad: cudaSetDevice");
     cudaStream_t st = (cudaStream_t)stream;

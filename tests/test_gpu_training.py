@@ -575,6 +575,53 @@ def test_logprobs_masks_and_ties(dtype, cols):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [3001, 40000, 152064])
+def test_top_of_rows_with_few_distinct_logits(dtype, cols):
+    """Masks that leave fewer tokens than asked for, ties at the last place in the first and last columns, and large
+    logits at periods that meet the kernel's groups of threads."""
+    low, g = torch.finfo(dtype).min, gen(2)
+    for n in (3, 40):
+        z = torch.full((n, cols), -math.inf, dtype=dtype, device=DEV)
+        for i in range(n):
+            kind = i % 8
+            if kind < 3:  # 0 to 24 tokens are left, masked by -inf, -1e4 or the lowest value
+                z[i] = (-math.inf, -1e4, low)[kind]
+                left = torch.randint(0, cols, (1 + (i * 5) % 24,), generator=g, device=DEV)
+                z[i, left] = torch.randn(len(left), generator=g, device=DEV).to(dtype)
+            elif kind == 3:
+                z[i] = 0.5
+                z[i, -40:] = 0.75  # the ties of the top are in the last columns
+            elif kind == 4:
+                z[i] = torch.randint(0, 3, (cols,), generator=g, device=DEV).to(dtype)
+            elif kind == 5:
+                z[i] = torch.randn(cols, generator=g, device=DEV).to(dtype)
+                z[i, 5::512] += 20  # one vector position of one group
+            elif kind == 6:
+                z[i] = 0
+                z[i, 8::1024], z[i, 9::1024] = 3, 4
+            else:
+                z[i, :] = 1
+                z[i, 1::2] = -math.inf
+        t = torch.zeros(n, dtype=torch.int64, device=DEV)
+        for top in (1, 5, 32):
+            check_logprobs(z, t, 0, top)
+            check_logprobs(z[:, 1:], t, 0, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_logprobs_and_gradient_of_minus_infinity_beside_very_low_logits(dtype):
+    """-inf has probability 0 even where the largest logit is the type's lowest value or not far from it."""
+    low = torch.finfo(dtype).min
+    tops = [low, low / 2, -1e4, -1e36, -1e37, -2e37, 1e36, 2e37, 1e38] if dtype != F16 else [low, -65000.0, -60032.0, -59000.0, 60000.0, 65000.0]
+    z = torch.full((len(tops), 4001), -math.inf, dtype=dtype, device=DEV)
+    for i, v in enumerate(tops):
+        z[i, i::7] = v
+    t = torch.arange(len(tops), device=DEV)
+    check_logprobs(z, t, 0, 3)
+    check_logprob_grad(z, t, 0, *grads_of(len(tops), 1))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_logprobs_of_nan_and_infinity(dtype):
     z = randn(4, 500, dtype=dtype, seed=1)
     z[0, 3], z[1, 4], z[2] = math.nan, math.inf, math.nan
