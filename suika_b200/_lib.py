@@ -230,6 +230,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_ext = None
 
 
 def library_path() -> str:
@@ -256,6 +257,16 @@ def load() -> C.CDLL:
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+def extension():
+    """The module _train (csrc/bind.cpp), which calls the library's training-step entries on torch tensors."""
+    global _ext
+    if _ext is None:
+        load()
+        from . import _train
+        _ext = _train
+    return _ext
 
 
 class ReshardError(RuntimeError):

@@ -10,15 +10,21 @@
 // bound once a few MB are moved. Below that the launches are.
 #include "train.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <utility>
 #include <vector>
+
+namespace cg = cooperative_groups;
 
 namespace {
 
 using namespace suika_train;
 
 constexpr int kThreads = 256;
+constexpr int kSmallThreads = 1024, kSmallCtas = 8;  // the cluster that sums a few MB
+constexpr uint64_t kSmallBytes = 1 << 20;
 
 struct SpanEnt {
   uint64_t ptr;
@@ -119,12 +125,11 @@ __device__ __forceinline__ double block_sum(double x) {
   return x;  // thread 0's is the sum
 }
 
-// One partial sum per CTA. The tiles of a CTA depend on the table and the grid alone and every sum
-// has a fixed order, so the same inputs give the same bits.
+// The sum over one CTA's tiles, as thread 0's result.
 template <int CAP>
-__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ SpanTable<CAP> t, double* partial) {
+__device__ __forceinline__ double tiles_sumsq(const SpanTable<CAP>& t, uint32_t first, uint32_t apart) {
   double acc = 0.0;
-  for (uint32_t tile = blockIdx.x; tile < t.n_tiles; tile += gridDim.x) {
+  for (uint32_t tile = first; tile < t.n_tiles; tile += apart) {
     const SpanEnt& e = t.e[find_entry(t.e, t.n, tile)];
     const uint32_t dt = e.dtype, isz = dt == RS_F32 ? 4 : 2, per = 16 / isz, most = t.tile_bytes / isz;
     const uint64_t off = (uint64_t)(tile - e.tile_begin) * most;
@@ -133,11 +138,11 @@ __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__
     const uint32_t head = min(len, (uint32_t)((16 - (p & 15)) & 15) / isz);
     const uint32_t nvec = (len - head) / per;
     const char* body = reinterpret_cast<const char*>(p + (uint64_t)head * isz);
-    for (uint32_t i = threadIdx.x; i < nvec; i += 4 * kThreads) {
+    for (uint32_t i = threadIdx.x; i < nvec; i += 4 * blockDim.x) {
       uint4 v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const uint32_t j = i + u * kThreads;
+        const uint32_t j = i + u * blockDim.x;
         v[u] = j < nvec ? ld16(body + (size_t)j * 16) : make_uint4(0, 0, 0, 0);
       }
       acc += batch_sumsq<4>(v, dt);
@@ -149,8 +154,32 @@ __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__
       acc = fma(x, x, acc);
     }
   }
-  acc = block_sum(acc);
+  return block_sum(acc);
+}
+
+// One partial sum per CTA. The tiles of a CTA depend on the table and the grid alone and every sum
+// has a fixed order, so the same inputs give the same bits.
+template <int CAP>
+__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ SpanTable<CAP> t, double* partial) {
+  const double acc = tiles_sumsq(t, blockIdx.x, gridDim.x);
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+// Up to 1 MB: one cluster, whose first CTA adds the others' sums from their shared memory: a launch less than
+// partial sums in memory take. (At 3 MB its 8 CTAs need 13 us, the two launches 8.)
+template <int CAP>
+__global__ void __launch_bounds__(kSmallThreads) sumsq_small_kernel(const __grid_constant__ SpanTable<CAP> t, double* sumsq) {
+  __shared__ double sums[kSmallCtas];
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();  // the first CTA runs before its memory is written
+  const double acc = tiles_sumsq(t, blockIdx.x, kSmallCtas);
+  if (threadIdx.x == 0) cluster.map_shared_rank(sums, 0)[blockIdx.x] = acc;
+  cluster.sync();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    double total = 0.0;
+    for (int i = 0; i < kSmallCtas; ++i) total += sums[i];
+    *sumsq = total;
+  }
 }
 
 constexpr int kFinishThreads = 1024;
@@ -373,6 +402,7 @@ int lay_tiles(Ent* e, int n, Tiles tiles, uint32_t* n_tiles) {
 
 constexpr uint32_t kRoundBytes = kThreads * 16;
 constexpr uint32_t kSumRounds = 8;     // 32 KB tiles, at most 64 CTAs to an SM: 7.04 TB/s; 8 CTAs to an SM 6.13
+constexpr uint32_t kSmallRounds = 16;  // one batch of loads of 1024 threads
 constexpr uint32_t kScaleRounds = 4;   // 16 KB tiles, one batch of loads: 6.85 TB/s; 32 KB 6.36
 constexpr uint32_t kUpdateRounds = 4;  // 8192 elements
 constexpr int kSumCtas = 64;           // per SM
@@ -424,6 +454,11 @@ int check_spans(const char* what, const rs_grad_span* spans, int64_t n, std::vec
   return RS_OK;
 }
 
+template <int CAP>
+auto sumsq_small_of(const SpanTable<CAP>&) -> void (*)(SpanTable<CAP>, double*) {
+  return sumsq_small_kernel<CAP>;
+}
+
 // Whether two of the ranges [begin, begin + bytes) share memory. Sorts them.
 bool any_overlap(std::vector<std::pair<uint64_t, uint64_t>>& r) {
   std::sort(r.begin(), r.end());
@@ -457,6 +492,22 @@ int rs_grad_sumsq(const rs_grad_span* spans, int64_t n, void* workspace, uint64_
     if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_grad_sumsq: cudaSetDevice");
     const int sms = std::min(sm_count(device), kMaxSms);
     cudaStream_t st = (cudaStream_t)stream;
+    uint64_t bytes = 0;
+    for (const rs_grad_span& g : s) bytes += g.numel * dtype_bytes(g.dtype);
+    if (bytes <= kSmallBytes && !s.empty() && s.size() <= (size_t)kSpanCaps[2])
+      return for_spans(s, 1, kSmallRounds, [&](const auto& t) -> int {  // eight tiles, or of 64 KB
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(kSmallCtas);
+        cfg.blockDim = dim3(kSmallThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = kSmallCtas;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        return tcuda(cudaLaunchKernelEx(&cfg, sumsq_small_of(t), t, sumsq_dev), "rs_grad_sumsq: launch (small)");
+      });
     double* partial = (double*)workspace;
     int used = 0;
     rc = for_spans(s, sms, kSumRounds, [&](const auto& t) -> int {

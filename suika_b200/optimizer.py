@@ -16,7 +16,6 @@ There is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -29,12 +28,6 @@ from .layouts import actual_shape, shard_spans
 DTYPE_CODES = {torch.float32: L.RS_F32, torch.bfloat16: L.RS_BF16, torch.float16: L.RS_F16}
 Grads = Union[Dict[str, torch.Tensor], Sequence[torch.Tensor]]
 Counted = Dict[str, List[Tuple[int, int]]]
-
-
-def raw_stream(device_index: int) -> int:
-    """The current stream's handle (torch.cuda.current_stream builds an object around it, which
-    costs as much as a small launch)."""
-    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def counted_spans(layout, rank: int) -> Counted:
@@ -79,81 +72,37 @@ def counted_spans(layout, rank: int) -> Counted:
     return out
 
 
-def _refuse(t: torch.Tensor, index: int, what: str) -> None:
-    """Raise for a tensor that the kernels do not take."""
-    if t.device.type != "cuda":
-        raise ValueError(f"{what} must be CUDA tensors")
-    if t.get_device() != index:
-        raise ValueError(f"{what} must share one device")
-    if not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
-    raise ValueError(f"{what} of {t.dtype}: float32, bfloat16 and float16 are taken")
+def _listed(grads: Grads) -> List[Optional[torch.Tensor]]:
+    return list(grads.values()) if hasattr(grads, "values") else list(grads)
 
 
-def _named(grads: Grads) -> Tuple[Optional[List[str]], List[torch.Tensor]]:
-    """(names or None, tensors); entries of None (a parameter without a gradient) are left out."""
-    if hasattr(grads, "items"):
-        kept = [(n, g) for n, g in grads.items() if g is not None]
-        names, tensors = [n for n, _ in kept], [g for _, g in kept]
-    else:
-        names, tensors = None, [g for g in grads if g is not None]
-    if not tensors:
-        raise ValueError("no gradients")
-    if tensors[0].device.type != "cuda":
-        raise ValueError("gradients must be CUDA tensors")
-    return names, tensors
-
-
-def _spans(tensors: List[torch.Tensor], what: str = "gradients"):
-    """(rs_grad_span array, its length) of whole tensors: one device, contiguous, a type the kernels take.
-    (A span is three 64-bit words, the type in the low half of the last.)"""
-    index = tensors[0].get_device()
-    words: List[int] = []
-    for t in tensors:
-        code = DTYPE_CODES.get(t.dtype)
-        if code is None or t.get_device() != index or not t.is_contiguous():
-            _refuse(t, index, what)
-        words += (t.data_ptr(), t.numel(), code)
-    return (C.c_uint64 * len(words))(*words), len(tensors)
-
-
-def _counted_spans(names: Optional[List[str]], tensors: List[torch.Tensor], counted: Counted):
-    if names is None:
+def _counted_parts(grads: Grads, counted: Counted) -> List[torch.Tensor]:
+    if not hasattr(grads, "items"):
         raise ValueError("counted spans go by name: give the gradients as {name: tensor}")
-    _spans(tensors)  # the checks
-    words: List[int] = []
-    for name, t in zip(names, tensors):
+    parts = []
+    for name, t in grads.items():
+        if t is None:
+            continue
         if name not in counted:
             raise AssertionError(f"no counted spans for {name}")
+        if not t.is_contiguous():
+            raise ValueError("gradients must be contiguous")
+        flat = t.detach().view(-1)
         for off, n in counted[name]:
             if off < 0 or n < 0 or off + n > t.numel():
                 raise AssertionError(f"{name}: counted span [{off}, {off + n}) leaves a gradient of {t.numel()} elements")
-            words += (t.data_ptr() + off * t.element_size(), n, DTYPE_CODES[t.dtype])
-    return (C.c_uint64 * len(words))(*words), len(words) // 3
-
-
-def _sumsq(spans, n: int, dev: torch.device) -> torch.Tensor:
-    lib = L.load()
-    nb = C.c_uint64()
-    L.check(lib.rs_grad_sumsq_workspace_bytes(n, C.byref(nb)))
-    workspace = torch.empty(nb.value, dtype=torch.uint8, device=dev)
-    out = torch.empty(1, dtype=torch.float64, device=dev)
-    L.check(lib.rs_grad_sumsq(spans, n, workspace.data_ptr(), nb.value, out.data_ptr(), dev.index, raw_stream(dev.index)))
-    return out
+            parts.append(flat[off:off + n])
+    return parts
 
 
 def grad_sumsq(grads: Grads, counted: Optional[Counted] = None) -> torch.Tensor:
     """Sum of squares of the gradients ({name: tensor} or a sequence; None entries are left out), a
     float64 tensor of one element on their device, summed in 64 bits. `counted` (counted_spans):
     only what this rank counts; then an all-reduce over the ranks gives the global sum."""
-    names, tensors = _named(grads)
-    spans, n = _spans(tensors) if counted is None else _counted_spans(names, tensors, counted)
-    return _sumsq(spans, n, tensors[0].device)
-
-
-def _check_sumsq(sumsq: torch.Tensor, dev: torch.device) -> None:
-    if sumsq.dtype != torch.float64 or sumsq.numel() != 1 or sumsq.device != dev:
-        raise ValueError("sumsq must be one float64 on the gradients' device")
+    if counted is None:
+        return L.extension().grad_sumsq(_listed(grads), None)
+    like = next((g for g in _listed(grads) if g is not None), None)
+    return L.extension().grad_sumsq(_counted_parts(grads, counted), like)
 
 
 def clip_grads(grads: Grads, max_norm: float, *, sumsq: Optional[torch.Tensor] = None, counted: Optional[Counted] = None,
@@ -165,18 +114,11 @@ def clip_grads(grads: Grads, max_norm: float, *, sumsq: Optional[torch.Tensor] =
     are refused. A norm that is not finite reaches the gradients, as in torch.nn.utils.clip_grad_norm_."""
     if not max_norm > 0:
         raise ValueError("max_norm must be positive")
-    names, tensors = _named(grads)
-    dev = tensors[0].device
-    spans, n = _spans(tensors)
-    if sumsq is None:
-        sumsq = _sumsq(*((spans, n) if counted is None else _counted_spans(names, tensors, counted)), dev)
+    if sumsq is None and (counted is not None or group is not None):
+        sumsq = grad_sumsq(grads, counted)
         if group is not None:
             dist.all_reduce(sumsq, group=group)
-    else:
-        _check_sumsq(sumsq, dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    L.check(L.load().rs_grad_clip(spans, n, sumsq.data_ptr(), max_norm, norm.data_ptr(), dev.index, raw_stream(dev.index)))
-    return norm
+    return L.extension().grad_clip(_listed(grads), max_norm, sumsq)
 
 
 class ShardAdamW:
@@ -190,9 +132,10 @@ class ShardAdamW:
     again with its count. Arithmetic is in 32 bits whatever the types (bias corrections in 64), one
     rounding per stored value.
 
-    no_decay: names whose weight decay is 0. max_norm: clip by the global norm; `counted` and `group`
-    as in clip_grads. lr, weight_decay and max_norm may be assigned between steps; a captured step
-    keeps those of its capture (the step counts live on the device and advance on replay).
+    The tensors that `state` holds when the optimizer is made are the ones it updates. no_decay: names
+    whose weight decay is 0. max_norm: clip by the global norm; `counted` and `group` as in
+    clip_grads. lr, weight_decay and max_norm may be assigned between steps; a captured step keeps
+    those of its capture (the step counts live on the device and advance on replay).
     """
 
     def __init__(self, state: Dict[str, Dict[str, torch.Tensor]], lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
@@ -212,10 +155,9 @@ class ShardAdamW:
         if unknown:
             raise ValueError(f"no_decay names that the state does not hold: {sorted(unknown)}")
         self.device = next(iter(state.values()))["param"].device if "param" in next(iter(state.values())) else None
-        table = np.zeros(len(self.names), dtype=L.ADAMW_TENSOR_DTYPE)
-        self._decays = np.ones(len(self.names), dtype=np.float32)
-        self._shapes = []
-        for i, name in enumerate(self.names):
+        self._fields = [[], [], [], [], []]  # param, master or None, exp_avg, exp_avg_sq, step of each name
+        self._decays = [0.0 if n in no_decay else 1.0 for n in self.names]
+        for name in self.names:
             ent = state[name]
             for s in ("param", "exp_avg", "exp_avg_sq", "step"):
                 if s not in ent:
@@ -224,9 +166,12 @@ class ShardAdamW:
             body = [t for t in (p, m, v, w) if t is not None]
             if self.device is None or self.device.type != "cuda":
                 raise ValueError(f"{name}'s sub-fields must be CUDA tensors")
-            for t in body:
-                if t.device != self.device or not t.is_contiguous() or t.dtype not in DTYPE_CODES:
-                    _refuse(t, self.device.index, f"{name}'s sub-fields")
+            if any(t.device != self.device for t in body):
+                raise ValueError(f"{name}'s sub-fields must share one device")
+            if not all(t.is_contiguous() for t in body):
+                raise ValueError(f"{name}'s sub-fields must be contiguous")
+            if p.dtype not in DTYPE_CODES:
+                raise ValueError(f"{name}'s param of {p.dtype}: float32, bfloat16 and float16 are taken")
             if any(t.shape != p.shape for t in body):
                 raise AssertionError(f"{name}'s sub-fields differ in shape")
             if m.dtype != v.dtype or m.dtype not in (torch.float32, torch.bfloat16):
@@ -238,22 +183,14 @@ class ShardAdamW:
                 raise AssertionError(f"{name}: a step of {step.numel()} elements")
             if step.dtype != torch.float32 or step.device != self.device:
                 step = ent["step"] = step.to(device=self.device, dtype=torch.float32)
-            table[i] = (0, p.data_ptr(), 0 if w is None else w.data_ptr(), m.data_ptr(), v.data_ptr(), step.data_ptr(), p.numel(), 0, 0,
-                        DTYPE_CODES[p.dtype], DTYPE_CODES[m.dtype])
-            self._shapes.append(p.shape)
-            if name in no_decay:
-                self._decays[i] = 0
-        self._table = table
+            for kept, t in zip(self._fields, (p, w, m, v, step)):
+                kept.append(t)
         self._check_disjoint()
 
     def _check_disjoint(self) -> None:
-        begin, size = [], []
-        for name in self.names:
-            for s, t in self.state[name].items():
-                if s in ("param", "master", "exp_avg", "exp_avg_sq", "step") and t is not None and t.numel():
-                    begin.append(t.data_ptr())
-                    size.append(t.numel() * t.element_size())
-        b, n = np.array(begin, np.uint64), np.array(size, np.uint64)
+        tensors = [t for kept in self._fields for t in kept if t is not None and t.numel()]
+        b = np.array([t.data_ptr() for t in tensors], np.uint64)
+        n = np.array([t.numel() * t.element_size() for t in tensors], np.uint64)
         order = np.argsort(b)
         if ((b + n)[order][:-1] > b[order][1:]).any():
             raise ValueError("sub-fields of the state share memory")
@@ -262,47 +199,13 @@ class ShardAdamW:
         """One update from {name: gradient}; names without a gradient (missing or None) stay as they are.
         Returns the norm before clipping (float32, on the device), or None without max_norm. `sumsq`:
         the global sum of squares, if the caller has it already."""
-        names, shapes, table, decays = self.names, self._shapes, self._table, self._decays
-        gs = [grads.get(n) for n in names]
-        if any(g is None for g in gs):
-            given = [g is not None for g in gs]
-            if not any(given):
-                raise ValueError("no gradients")
-            names, gs, shapes = ([x for x, k in zip(xs, given) if k] for xs in (names, gs, shapes))
-            table, decays = table[given], decays[given]
-        if len(grads) > len(gs):
+        gs = [grads.get(n) for n in self.names]
+        if len(grads) > len(gs) or any(g is None for g in gs):
             extra = [n for n, g in grads.items() if g is not None and n not in self.state]
             if extra:
                 raise AssertionError(f"gradients of names that the state does not hold: {extra[:3]}")
-        dev = self.device
-        index = dev.index
-        at: List[int] = []
-        codes: List[int] = []
-        for n, g, shape in zip(names, gs, shapes):
-            code = DTYPE_CODES.get(g.dtype)
-            if code is None or g.get_device() != index or not g.is_contiguous():
-                _refuse(g, index, "gradients")
-            if g.shape != shape:
-                raise AssertionError(f"{n}: a gradient of another shape")
-            at.append(g.data_ptr())
-            codes.append(code)
-        lib = L.load()
-        norm = None
-        if self.max_norm is not None:
-            if sumsq is None:
-                sumsq = _sumsq(*(_spans(gs) if self.counted is None else _counted_spans(names, gs, self.counted)), dev)
-                if self.group is not None:
-                    dist.all_reduce(sumsq, group=self.group)
-            else:
-                _check_sumsq(sumsq, dev)
-            norm = torch.empty((), dtype=torch.float32, device=dev)
-        table["grad_dev"] = at
-        table["grad_dtype"] = codes
-        table["weight_decay"] = decays * np.float32(self.weight_decay)
-        opts = L.RsAdamwOpts(self.lr, self.betas[0], self.betas[1], self.eps, self.max_norm or 0.0)
-        nb = C.c_uint64()
-        L.check(lib.rs_adamw_workspace_bytes(len(table), C.byref(nb)))
-        workspace = torch.empty(nb.value, dtype=torch.uint8, device=dev)
-        L.check(lib.rs_adamw_step(table.ctypes.data, len(table), C.byref(opts), None if norm is None else sumsq.data_ptr(),
-                                  None if norm is None else norm.data_ptr(), workspace.data_ptr(), nb.value, index, raw_stream(index)))
-        return norm
+        if self.max_norm is not None and sumsq is None and (self.counted is not None or self.group is not None):
+            sumsq = grad_sumsq({n: g for n, g in zip(self.names, gs)}, self.counted)
+            if self.group is not None:
+                dist.all_reduce(sumsq, group=self.group)
+        return L.extension().adamw_step(*self._fields, self._decays, gs, self.lr, *self.betas, self.eps, self.weight_decay, self.max_norm, sumsq)
