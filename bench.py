@@ -15,7 +15,8 @@ target tensors); the time of a step is the max over ranks of the device time.
 Other modes (not the driver's contract lines): --impl reference-nccl (the reference's own GPU
 path, execute_param_transfer over NCCL, on the N > 1 workload), --handoff (old -> new process
 hand-off, 1 GPU), --activation (pipeline activation hand-over, N >= 2), --metadata (layout
-exchange and planning, any N; gloo without GPUs), --fanout (DP-replica fan-out of the push path).
+exchange and planning, any N; gloo without GPUs), --fanout (DP-replica fan-out of the push path),
+--next-step (reshard, then one clipped AdamW update of every target rank's state, 1 GPU).
 """
 from __future__ import annotations
 
@@ -739,6 +740,8 @@ def main():
     ap.add_argument("--checkpoint", action="store_true",
                     help="time checkpoint resume instead: one target rank's state built on the GPU from host shards "
                          "(1 GPU; ours against the reference's CPU execute plus a copy to the GPU)")
+    ap.add_argument("--next-step", action="store_true",
+                    help="time one clipped AdamW update of every target rank's state after a reshard instead (1 GPU)")
     ap.add_argument("--peer-probe", action="store_true",
                     help="time the copy kernel's peer patterns between GPU 0 and GPU 1 instead (one process, 2 GPUs)")
     ap.add_argument("--peer-gib", type=float, default=2.0)
@@ -758,6 +761,9 @@ def main():
         return
     if args.checkpoint:
         print(json.dumps(run_checkpoint(args)), flush=True)
+        return
+    if args.next_step:
+        print(json.dumps(run_next_step(args)), flush=True)
         return
     if args.warmup < 3:
         raise SystemExit("--warmup must be >= 3")
@@ -883,6 +889,51 @@ def run_checkpoint(args):
             "check": {"byte_equal": bool(same)},
             "reference_path": "oracle/nccl_port.checkpoint_rank (execute on device cpu, Suika/migration.py:1235-1244) + .to(cuda)",
             "host_threads": torch.get_num_threads()}
+
+
+# ---------------------------------------------------------------------------------------------
+# --next-step: the optimizer step of the state a reshard moved (1 GPU)
+# ---------------------------------------------------------------------------------------------
+def run_next_step(args):
+    """The step a job takes after its reshard: cfg2b on a layer sample (every target rank's state on one GPU, resharded by
+    reshard_local), then, per rank, the global gradient norm (each replicated tensor counted once), clipping and
+    AdamW on the master with bf16 gradients. Beside it torch's own: clip_grad_norm_ and AdamW(foreach) on the
+    masters and fp32 gradients, then the bf16 parameters copied from the masters. Device time, CUDA events; the
+    state and gradients are larger than L2."""
+    from suika_b200 import optimizer as OPT
+    dev = torch.device("cuda", 0)
+    torch.cuda.set_device(dev)
+    cfg = workload(1, args.layers or 4)
+    spl, tpl = cfg.layouts()
+    src = S.DeviceState(spl.layout[0], dev)
+    states = M.reshard_local(spl, tpl, {0: src.state}, S.expected_sub_fields(), dev)
+    del src
+    counted = {r: OPT.counted_spans(tpl, r) for r in states}
+    grads = {r: {n: torch.randn_like(e["param"]) for n, e in st.items()} for r, st in states.items()}
+    opts = {r: OPT.ShardAdamW(st, lr=1e-4, weight_decay=0.1, max_norm=1.0) for r, st in states.items()}
+    elements = sum(e["param"].numel() for st in states.values() for e in st.values())
+
+    def ours():
+        total = sum(OPT.grad_sumsq(g, counted[r]) for r, g in grads.items())
+        for r, o in opts.items():
+            o.step(grads[r], sumsq=total)
+    t_ours = _median_event_s(ours, args.steps)
+    params = [torch.nn.Parameter(e["master"]) for st in states.values() for e in st.values()]
+    for p, g in zip(params, (g for gs in grads.values() for g in gs.values())):
+        p.grad = g.float()
+    adam = torch.optim.AdamW(params, lr=1e-4, weight_decay=0.1, foreach=True)
+    bf16 = [e["param"] for st in states.values() for e in st.values()]
+
+    def torchs():
+        torch.nn.utils.clip_grad_norm_(params, 1.0, foreach=True)
+        adam.step()
+        torch._foreach_copy_(bf16, [p.detach() for p in params])
+    t_torch = _median_event_s(torchs, args.steps)
+    nbytes = elements * (2 + 12 + 12 + 2)
+    return {"metric": "clipped AdamW update of a resharded training state", "value": round(nbytes / t_ours / 1e9, 1), "unit": "GB/s",
+            "n_gpus": 1, "steps": args.steps, "ms_per_step": round(t_ours * 1e3, 3), "higher_is_better": True, "data": "synthetic",
+            "config": {"workload": f"{cfg.note}, {cfg.spec.n_layers} layers, both target ranks on one GPU; bf16 gradients, fp32 master and moments"},
+            "elements": elements, "torch_foreach_ms_per_step": round(t_torch * 1e3, 3), "speedup": round(t_torch / t_ours, 2)}
 
 
 # ---------------------------------------------------------------------------------------------

@@ -6,6 +6,8 @@ reshard_local (all ranks of a reshard emulated on one device). Around them:
   suika_b200.handoff     old -> new process hand-off (Suika/utils.py:325-406)
   suika_b200.metadata    layouts exchanged as planner records (Suika/migration.py:172-192)
   suika_b200.activation  activation hand-over between pipeline stages (Suika/pipeline_parallel.py:665-836)
+  suika_b200.optimizer   gradient norm, clipping and AdamW on a rank's shards (tasks/task.py:72-73)
+  suika_b200.vocab       embedding and token log probabilities of a vocabulary shard
 """
 from .migration import (ParamLayout, Plan, Program, TensorMeta, TransferOp, get_param_tensor_meta,  # noqa: F401
                         is_ib_enabled, launch_copies)

@@ -70,6 +70,11 @@ int64_t integer(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) already_set();
   return v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) already_set();
+  return v != 0;
+}
 std::string type_name(const at::Tensor& t) { return c10::toString(t.scalar_type()); }
 
 int code_of(const at::Tensor& t) {
@@ -147,7 +152,7 @@ PyObject* embed_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor ids = index_tensor(tensor(a[1], "ids"), grad_out, "ids");
     if (grad_out.sizes().slice(0, grad_out.dim() - 1) != ids.sizes())
       assertion_error("grad_out has shape " + shape_of(grad_out.sizes()) + ", ids " + shape_of(ids.sizes()));
-    o.accumulate = PyObject_IsTrue(a[7]) == 1;
+    o.accumulate = truth(a[7]);
     const bool has_dtype = a[5] != Py_None;
     if (has_dtype && !THPDtype_Check(a[5])) throw Raise{PyExc_TypeError, "dtype must be a torch.dtype"};
     const at::ScalarType dtype = has_dtype ? reinterpret_cast<THPDtype*>(a[5])->scalar_type : grad_out.scalar_type();
@@ -257,7 +262,7 @@ PyObject* token_logprobs_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return entry([&]() -> PyObject* {
     count_args("token_logprobs_grad", n, 10);
     const at::Tensor& logits = tensor(a[0], "logits");
-    const Logits l(logits, tensor(a[1], "targets"), 0, integer(a[7]), PyObject_IsTrue(a[8]) == 1);
+    const Logits l(logits, tensor(a[1], "targets"), 0, integer(a[7]), truth(a[8]));
     if (a[5] != Py_None && a[3] == Py_None) value_error("a gradient of the entropy needs the entropy");
     if (a[2] == Py_None || a[4] == Py_None) value_error("lse and grad_logprob are needed");
     static const char* names[5] = {"lse", "entropy", "grad_logprob", "grad_entropy", "grad_lse"};

@@ -10,7 +10,9 @@ on the vocabulary rows [lo, lo + rows) that its TensorMeta gives it (shard_range
     top alternatives from one pass over the logits; over several shards (`group`) each rank sends a
     record of 4 + 2 top floats per row, not its logits.
 embedding and token_logprobs are differentiable (torch.autograd). Every call is stream-ordered on the
-current stream of the tensors' device and can be captured. There is no CPU path.
+current stream of the tensors' device and can be captured into a CUDA graph. To capture a backward
+pass, call embedding_grad and token_logprobs_grad: torch's autograd engine cannot be captured while
+an eager graph of the same leaves lives. There is no CPU path.
 """
 from __future__ import annotations
 
@@ -137,9 +139,9 @@ def _forward(logits, targets, top, lo, group, starts):
     if starts is None:  # equal shards in rank order
         starts = [lo + (r - dist.get_rank(group)) * cols for r in range(world)]
     mine = L.extension().token_record(logits, targets, top, lo)
-    everyone = torch.empty((world, *mine.shape), dtype=mine.dtype, device=mine.device)
+    everyone = torch.empty((world * mine.shape[0], mine.shape[1]), dtype=mine.dtype, device=mine.device)
     dist.all_gather_into_tensor(everyone, mine, group=group)
-    r = merge_token_records(everyone, starts)
+    r = merge_token_records(everyone.view(world, *mine.shape), starts)
     return tuple(None if t is None else t.reshape(*targets.shape, *t.shape[1:]) for t in r)
 
 
@@ -186,6 +188,8 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.
                         grad_lse: Optional[torch.Tensor] = None, lo: int = 0, sharded: bool = False,
                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gradient of token_logprobs' logits, in their shape and type, from the gradients of logprob,
-    entropy and lse (float32). lse and entropy are token_logprobs' own. sharded=True: the logits are
-    one of several shards, and a target outside it is another's. `out` may be the logits themselves."""
+    entropy and lse (float32). lse and entropy are token_logprobs' own. `out` may be the logits themselves.
+    sharded=True: the logits are one of several shards, and a target outside it is another's; probabilities
+    then come from lse alone, whose 32 bits leave them off by |lse| 2^-24 (a whole row with |lse| over
+    1024 has its maximum and sum taken again)."""
     return L.extension().token_logprobs_grad(logits, targets, lse, entropy, grad_logprob, grad_entropy, grad_lse, lo, sharded, out)
