@@ -466,12 +466,12 @@ typedef struct rs_adamw_opts {
   double beta1;
   double beta2;
   double eps;
-  double max_norm; /* used when sumsq_dev is given */
+  double max_norm; /* 0: no clipping */
 } rs_adamw_opts;
 
-/* step += 1 and one AdamW update of every tensor. sumsq_dev (or NULL: no clipping): the gradients count
- * times min(1, max_norm / (sqrt(*sumsq_dev) + 1e-6)) without being written, and the norm goes to norm_dev
- * (may be NULL). No two tensors may share memory. */
+/* step += 1 and one AdamW update of every tensor. With max_norm > 0 the gradients count times
+ * min(1, max_norm / (norm + 1e-6)) without being written, and the norm goes to norm_dev (may be NULL): sqrt(*sumsq_dev)
+ * where that is given, else the norm of these gradients. No two tensors may share memory. */
 int rs_adamw_workspace_bytes(int64_t n_tensors, uint64_t* bytes);
 int rs_adamw_step(const rs_adamw_tensor* tensors, int64_t n_tensors, const rs_adamw_opts* opts, const double* sumsq_dev,
                   float* norm_dev, void* workspace_dev, uint64_t workspace_bytes, int32_t device, void* stream);

@@ -404,14 +404,17 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool clip = a[12] != Py_None;
     if (clip) {
       o.max_norm = number(a[12]);
-      sumsq = a[13] == Py_None ? sumsq_of(spans_of(ts), first) : tensor(a[13], "sumsq");
-      given_sumsq(sumsq, first);
+      if (!(o.max_norm > 0)) value_error("max_norm must be positive");
+      if (a[13] != Py_None) {
+        sumsq = tensor(a[13], "sumsq");
+        given_sumsq(sumsq, first);
+      }
       norm = at::empty({}, first.options().dtype(at::kFloat));
     }
     uint64_t bytes = 0;
     check(rs_adamw_workspace_bytes((int64_t)t.size(), &bytes));
     const at::Tensor workspace = at::empty({(int64_t)bytes}, first.options().dtype(at::kByte));
-    check(rs_adamw_step(t.data(), (int64_t)t.size(), &o, clip ? sumsq.data_ptr<double>() : nullptr, clip ? norm.data_ptr<float>() : nullptr,
+    check(rs_adamw_step(t.data(), (int64_t)t.size(), &o, sumsq.defined() ? sumsq.data_ptr<double>() : nullptr, clip ? norm.data_ptr<float>() : nullptr,
                         workspace.data_ptr(), bytes, first.get_device(), stream_of(first)));
     return clip ? THPVariable_Wrap(std::move(norm)) : Py_NewRef(Py_None);
   });

@@ -116,6 +116,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_fill_kernel(SortArgs a) {
   uint2* buf = reinterpret_cast<uint2*>(smem);                    // CAP pairs
   uint16_t(*cnt)[kBins] = reinterpret_cast<uint16_t(*)[kBins]>(buf + CAP);  // per warp and digit, at most 32 * R
   __shared__ uint32_t total[kBins], base[kBins], scan[kBins / 32];
+  let_successor_start();
   cg::cluster_group cluster = cg::this_cluster();
   const int cs = cluster.num_blocks();
   if (blockIdx.x >= cs) {  // not in the sorting cluster
@@ -242,6 +243,8 @@ __device__ __forceinline__ void store_out(G* out, int64_t at, const float* x) {
 // an fp32 gradient: 155 us, 174 and 209).
 template <class T, class G, int E, bool ACC>
 __global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* out, int64_t units) {
+  let_successor_start();
+  after_predecessor();
   constexpr int NV = kCols / E;
   const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (unit >= units) return;
@@ -351,6 +354,7 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* o
 // of consecutive pieces in order, and the runs are added in order: the same bits always.
 template <class G, int V>
 __global__ void __launch_bounds__(256) join_kernel(SumArgs a, G* out, bool accumulate) {
+  after_predecessor();
   using P = Pack<float, V>;
   __shared__ P sums[8][32];
   const int chunks = (a.hidden + 32 * V - 1) / (32 * V), lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -479,21 +483,19 @@ int launch_sums(const SumArgs& a, const GradPlan& p, const void* grad, void* out
   const unsigned grid = (unsigned)((units + 7) / 8);
   auto go = [&](auto E) {
     constexpr int EE = decltype(E)::value;
-    if (accumulate) sum_kernel<T, G, EE, true><<<grid, 256, 0, st>>>(a, (const T*)grad, (G*)out, units);
-    else sum_kernel<T, G, EE, false><<<grid, 256, 0, st>>>(a, (const T*)grad, (G*)out, units);
+    return launch_after(accumulate ? sum_kernel<T, G, EE, true> : sum_kernel<T, G, EE, false>, grid, 256, st, a, (const T*)grad, (G*)out, units);
   };
-  if (e == 8) { if constexpr (sizeof(T) == 2) go(std::integral_constant<int, 8>{}); }
-  else if (e == 4) go(std::integral_constant<int, 4>{});
-  else if (e == 2) go(std::integral_constant<int, 2>{});
-  else go(std::integral_constant<int, 1>{});
-  int rc = tcuda(cudaGetLastError(), "rs_embed_grad: launch (sums)");
+  cudaError_t launched = cudaErrorInvalidValue;
+  if (e == 8) { if constexpr (sizeof(T) == 2) launched = go(std::integral_constant<int, 8>{}); }
+  else if (e == 4) launched = go(std::integral_constant<int, 4>{});
+  else if (e == 2) launched = go(std::integral_constant<int, 2>{});
+  else launched = go(std::integral_constant<int, 1>{});
+  int rc = tcuda(launched, "rs_embed_grad: launch (sums)");
   if (rc != RS_OK || p.tiles < 2) return rc;  // one tile has no row longer than a tile
   const int v = a.hidden % 4 == 0 ? 4 : 1;  // columns per lane
   const int64_t most = (int64_t)(p.tiles - 1) * ((a.hidden + 32 * v - 1) / (32 * v));
   const unsigned ctas = (unsigned)std::min<int64_t>(most, (int64_t)sms * 8);
-  if (v == 4) join_kernel<G, 4><<<ctas, 256, 0, st>>>(a, (G*)out, accumulate);
-  else join_kernel<G, 1><<<ctas, 256, 0, st>>>(a, (G*)out, accumulate);
-  return tcuda(cudaGetLastError(), "rs_embed_grad: launch (join)");
+  return tcuda(launch_after(v == 4 ? join_kernel<G, 4> : join_kernel<G, 1>, ctas, 256, st, a, (G*)out, accumulate), "rs_embed_grad: launch (join)");
 }
 
 template <class T>

@@ -161,6 +161,7 @@ __device__ __forceinline__ double tiles_sumsq(const SpanTable<CAP>& t, uint32_t 
 // has a fixed order, so the same inputs give the same bits.
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ SpanTable<CAP> t, double* partial) {
+  let_successor_start();
   const double acc = tiles_sumsq(t, blockIdx.x, gridDim.x);
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
@@ -184,6 +185,7 @@ __global__ void __launch_bounds__(kSmallThreads) sumsq_small_kernel(const __grid
 
 constexpr int kFinishThreads = 1024;
 __global__ void __launch_bounds__(kFinishThreads) sumsq_finish_kernel(const double* partial, int n, double* sumsq) {
+  after_predecessor();
   double acc = 0.0;
   for (int i = threadIdx.x; i < n; i += kFinishThreads) acc += partial[i];
   acc = block_sum(acc);
@@ -202,6 +204,7 @@ __device__ __forceinline__ float clip_factor(double sumsq, float max_norm, float
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ SpanTable<CAP> t, const double* sumsq,
                                                          float max_norm, float* norm_out) {
+  after_predecessor();
   float norm;
   const float c = clip_factor(*sumsq, max_norm, &norm);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
@@ -274,13 +277,23 @@ struct PrepTable {
 // (1 - beta^t loses digits in 32). One thread per tensor, so no CTA of the update reads a step that
 // another one advances. {lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr * wd, clip factor}.
 template <int CAP>
-__global__ void __launch_bounds__(kThreads) prep_kernel(const __grid_constant__ PrepTable<CAP> t, const double* sumsq,
+__global__ void __launch_bounds__(kThreads) prep_kernel(const __grid_constant__ PrepTable<CAP> t, const double* partial, int n_partial,
                                                         float max_norm, float* norm_out, float4* scal) {
+  let_successor_start();
+  after_predecessor();
+  __shared__ float factor;
   float c = 1.f;
-  if (sumsq) {
-    float norm;
-    c = clip_factor(*sumsq, max_norm, &norm);
-    if (norm_out && threadIdx.x == 0) *norm_out = norm;
+  if (n_partial) {  // the sum of squares, in one piece or in the norm's partial sums
+    double sumsq = 0.0;
+    for (int i = threadIdx.x; i < n_partial; i += kThreads) sumsq += partial[i];
+    sumsq = block_sum(sumsq);
+    if (threadIdx.x == 0) {
+      float norm;
+      factor = clip_factor(sumsq, max_norm, &norm);
+      if (norm_out) *norm_out = norm;
+    }
+    __syncthreads();
+    c = factor;
   }
   for (int i = threadIdx.x; i < t.n; i += kThreads) {
     float* sp = reinterpret_cast<float*>(t.e[i].step);
@@ -341,6 +354,7 @@ __device__ __forceinline__ void store8(uint64_t base, uint64_t i, uint32_t dt, c
 // over the CTA), so one launch takes tables of mixed types.
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ AdamTable<CAP> t, const float4* scal) {
+  after_predecessor();
   const AdamHyper h{t.beta2, t.one_minus_beta1, t.one_minus_beta2, t.eps};
   const uint32_t tile = t.n_tiles - 1 - blockIdx.x;  // last tile first: the norm's pass left those gradients in L2
   const int k = find_entry(t.e, t.n, tile);
@@ -459,6 +473,26 @@ auto sumsq_small_of(const SpanTable<CAP>&) -> void (*)(SpanTable<CAP>, double*) 
   return sumsq_small_kernel<CAP>;
 }
 
+template <int CAP>
+auto scale_of(const SpanTable<CAP>&) -> void (*)(SpanTable<CAP>, const double*, float, float*) {
+  return scale_kernel<CAP>;
+}
+
+// The partial sums of the norm's pass, one for each CTA; *used of them.
+int launch_partials(const std::vector<rs_grad_span>& s, int sms, double* partial, int* used, cudaStream_t st) {
+  *used = 0;
+  return for_spans(s, sms, kSumRounds, [&](const auto& t) -> int {
+    const int grid = (int)std::min<uint64_t>(t.n_tiles, (uint64_t)sms * kSumCtas);
+    sumsq_kernel<<<grid, kThreads, 0, st>>>(t, partial + *used);
+    *used += grid;
+    return tcuda(cudaGetLastError(), "the norm's launch");
+  });
+}
+uint64_t partial_bytes(int64_t n_spans) {
+  const uint64_t launches = std::max<uint64_t>(1, ((uint64_t)n_spans + kSpanCaps[2] - 1) / kSpanCaps[2]);
+  return launches * kSumCtas * kMaxSms * sizeof(double);
+}
+
 // Whether two of the ranges [begin, begin + bytes) share memory. Sorts them.
 bool any_overlap(std::vector<std::pair<uint64_t, uint64_t>>& r) {
   std::sort(r.begin(), r.end());
@@ -473,8 +507,7 @@ extern "C" {
 
 int rs_grad_sumsq_workspace_bytes(int64_t n_spans, uint64_t* bytes) {
   if (n_spans < 0 || !bytes) return tfail(RS_ERR_ARG, "rs_grad_sumsq_workspace_bytes: bad argument");
-  const uint64_t launches = std::max<uint64_t>(1, ((uint64_t)n_spans + kSpanCaps[2] - 1) / kSpanCaps[2]);
-  *bytes = launches * kSumCtas * kMaxSms * sizeof(double);
+  *bytes = partial_bytes(n_spans);
   return RS_OK;
 }
 
@@ -510,15 +543,8 @@ int rs_grad_sumsq(const rs_grad_span* spans, int64_t n, void* workspace, uint64_
       });
     double* partial = (double*)workspace;
     int used = 0;
-    rc = for_spans(s, sms, kSumRounds, [&](const auto& t) -> int {
-      const int grid = (int)std::min<uint64_t>(t.n_tiles, (uint64_t)sms * kSumCtas);
-      sumsq_kernel<<<grid, kThreads, 0, st>>>(t, partial + used);
-      used += grid;
-      return tcuda(cudaGetLastError(), "rs_grad_sumsq: launch");
-    });
-    if (rc != RS_OK) return rc;
-    sumsq_finish_kernel<<<1, kFinishThreads, 0, st>>>(partial, used, sumsq_dev);
-    return tcuda(cudaGetLastError(), "rs_grad_sumsq: launch (finish)");
+    if ((rc = launch_partials(s, sms, partial, &used, st)) != RS_OK) return rc;
+    return tcuda(launch_after(sumsq_finish_kernel, 1, kFinishThreads, st, partial, used, sumsq_dev), "rs_grad_sumsq: launch (finish)");
   });
 }
 
@@ -540,19 +566,17 @@ int rs_grad_clip(const rs_grad_span* spans, int64_t n, const double* sumsq_dev, 
     cudaStream_t st = (cudaStream_t)stream;
     if (s.empty()) {  // no elements here: the norm alone
       SpanTable<kSpanCaps[0]> t{};
-      scale_kernel<<<1, kThreads, 0, st>>>(t, sumsq_dev, max_norm, norm_dev);
-      return tcuda(cudaGetLastError(), "rs_grad_clip: launch");
+      return tcuda(launch_after(scale_kernel<kSpanCaps[0]>, 1, kThreads, st, t, sumsq_dev, max_norm, norm_dev), "rs_grad_clip: launch");
     }
     return for_spans(s, sms, kScaleRounds, [&](const auto& t) -> int {
-      scale_kernel<<<t.n_tiles, kThreads, 0, st>>>(t, sumsq_dev, max_norm, norm_dev);
-      return tcuda(cudaGetLastError(), "rs_grad_clip: launch");
+      return tcuda(launch_after(scale_of(t), t.n_tiles, kThreads, st, t, sumsq_dev, max_norm, norm_dev), "rs_grad_clip: launch");
     });
   });
 }
 
 int rs_adamw_workspace_bytes(int64_t n_tensors, uint64_t* bytes) {
   if (n_tensors < 0 || !bytes) return tfail(RS_ERR_ARG, "rs_adamw_workspace_bytes: bad argument");
-  *bytes = std::max<uint64_t>(1, (uint64_t)n_tensors) * sizeof(float4);
+  *bytes = (std::max<uint64_t>(1, (uint64_t)n_tensors) * sizeof(float4) + 255) / 256 * 256 + partial_bytes(n_tensors);
   return RS_OK;
 }
 
@@ -561,8 +585,8 @@ int rs_adamw_workspace_bytes(int64_t n_tensors, uint64_t* bytes) {
 namespace {
 
 template <int CAP>
-int adam_chunk(const rs_adamw_tensor* a, int n, const rs_adamw_opts& o, const double* sumsq, float* norm_out, float4* scal,
-               int sms, cudaStream_t st) {
+int adam_chunk(const rs_adamw_tensor* a, int n, const rs_adamw_opts& o, const double* partial, int n_partial, float* norm_out,
+               float4* scal, int sms, cudaStream_t st) {
   PrepTable<CAP> p;
   AdamTable<CAP> t;
   uint64_t total = 0;
@@ -582,11 +606,9 @@ int adam_chunk(const rs_adamw_tensor* a, int n, const rs_adamw_opts& o, const do
   t.tile = tile_rounds(total / (kThreads * 8), sms, kUpdateRounds) * kThreads * 8;
   int rc = lay_tiles(t.e, n, [&](int i) { return (a[i].numel + t.tile - 1) / t.tile; }, &t.n_tiles);
   if (rc != RS_OK) return rc;
-  prep_kernel<<<1, kThreads, 0, st>>>(p, sumsq, (float)o.max_norm, norm_out, scal);
-  if ((rc = tcuda(cudaGetLastError(), "rs_adamw_step: launch (factors)")) != RS_OK) return rc;
-  if (t.n_tiles == 0) return RS_OK;
-  adamw_kernel<<<t.n_tiles, kThreads, 0, st>>>(t, scal);
-  return tcuda(cudaGetLastError(), "rs_adamw_step: launch");
+  rc = tcuda(launch_after(prep_kernel<CAP>, 1, kThreads, st, p, partial, n_partial, (float)o.max_norm, norm_out, scal), "rs_adamw_step: launch (factors)");
+  if (rc != RS_OK || t.n_tiles == 0) return rc;
+  return tcuda(launch_after(adamw_kernel<CAP>, t.n_tiles, kThreads, st, t, (const float4*)scal), "rs_adamw_step: launch");
 }
 
 }  // namespace
@@ -598,7 +620,7 @@ extern "C" int rs_adamw_step(const rs_adamw_tensor* tensors, int64_t n, const rs
     const rs_adamw_opts& o = *opts;
     if (!(o.beta1 >= 0 && o.beta1 < 1 && o.beta2 >= 0 && o.beta2 < 1 && o.eps >= 0 && o.lr >= 0))
       return tfail(RS_ERR_ARG, "rs_adamw_step: lr, betas or eps out of range");
-    if (sumsq_dev && !(o.max_norm > 0)) return tfail(RS_ERR_ARG, "rs_adamw_step: max_norm must be positive");
+    if (sumsq_dev ? !(o.max_norm > 0) : !(o.max_norm >= 0)) return tfail(RS_ERR_ARG, "rs_adamw_step: max_norm must be positive");
     if (n == 0) return RS_OK;
     for (int64_t i = 0; i < n; ++i) {
       const rs_adamw_tensor& a = tensors[i];
@@ -618,14 +640,30 @@ extern "C" int rs_adamw_step(const rs_adamw_tensor* tensors, int64_t n, const rs
       return tfail(RS_ERR_CAPACITY, "rs_adamw_step: workspace too small or not 16-byte aligned");
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_adamw_step: cudaSetDevice");
-    const int sms = sm_count(device);
+    const int sms = std::min(sm_count(device), kMaxSms);
     cudaStream_t st = (cudaStream_t)stream;
     float4* scal = (float4*)workspace;
+    const double* partial = sumsq_dev;
+    int n_partial = sumsq_dev ? 1 : 0;
+    if (!sumsq_dev && o.max_norm > 0) {  // the norm of these gradients; the factors' launch adds the partial sums
+      std::vector<rs_grad_span> s;
+      s.reserve((size_t)n);
+      for (int64_t i = 0; i < n; ++i)
+        if (tensors[i].numel) s.push_back({tensors[i].grad_dev, tensors[i].numel, tensors[i].grad_dtype, 0});
+      double* sums = (double*)((char*)workspace + (need - partial_bytes(n)));
+      int rc = launch_partials(s, sms, sums, &n_partial, st);
+      if (rc != RS_OK) return rc;
+      if (n_partial == 0) {  // no elements: the norm is 0
+        if ((rc = tcuda(cudaMemsetAsync(sums, 0, sizeof(double), st), "rs_adamw_step: cudaMemsetAsync")) != RS_OK) return rc;
+        n_partial = 1;
+      }
+      partial = sums;
+    }
     for (int64_t i = 0; i < n; i += 560) {
       const int c = (int)std::min<int64_t>(n - i, 560);
-      int rc = c <= 16 ? adam_chunk<16>(tensors + i, c, o, sumsq_dev, norm_dev, scal + i, sms, st)
-             : c <= 96 ? adam_chunk<96>(tensors + i, c, o, sumsq_dev, norm_dev, scal + i, sms, st)
-                       : adam_chunk<560>(tensors + i, c, o, sumsq_dev, norm_dev, scal + i, sms, st);
+      int rc = c <= 16 ? adam_chunk<16>(tensors + i, c, o, partial, n_partial, norm_dev, scal + i, sms, st)
+             : c <= 96 ? adam_chunk<96>(tensors + i, c, o, partial, n_partial, norm_dev, scal + i, sms, st)
+                       : adam_chunk<560>(tensors + i, c, o, partial, n_partial, norm_dev, scal + i, sms, st);
       if (rc != RS_OK) return rc;
     }
     return RS_OK;

@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <exception>
 #include <string>
+#include <utility>
 
 namespace suika_train {
 
@@ -65,7 +66,30 @@ int guarded(const char* what, F&& body) {
   }
 }
 
+// Launches a kernel that follows another of the same call on the stream: it may be set up while its
+// predecessor runs out (programmatic dependent launch), and begins with after_predecessor().
+template <class... P, class... A>
+cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
+
 // ---- device side --------------------------------------------------------------------------
+
+// Waits until the kernel before this one has ended and its stores are visible. Every thread of a kernel
+// launched by launch_after calls it first, also one that has nothing to do: the next kernel takes
+// the end of this one for the end of both.
+__device__ __forceinline__ void after_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next kernel's CTAs be set up as soon as every CTA of this one has begun to end.
+__device__ __forceinline__ void let_successor_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // 16 bytes that this launch reads once (no L1 line is kept for them).
 __device__ __forceinline__ uint4 ld16(const void* p) {
