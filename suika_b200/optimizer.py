@@ -132,7 +132,8 @@ class ShardAdamW:
     again with its count. Arithmetic is in 32 bits whatever the types (bias corrections in 64), one
     rounding per stored value.
 
-    The tensors that `state` holds when the optimizer is made are the ones it updates. no_decay: names
+    The tensors that `state` holds when the optimizer is made are the ones it updates; states that view
+    one source (reshard_local with views=True) must not each be stepped. no_decay: names
     whose weight decay is 0. max_norm: clip by the global norm; `counted` and `group` as in
     clip_grads. lr, weight_decay and max_norm may be assigned between steps; a captured step keeps
     those of its capture (the step counts live on the device and advance on replay).

@@ -434,6 +434,25 @@ def test_embedding_grad_key_widths(rows):
     check_grad(randn(1500, 16, seed=rows), spread("distinct", 1500, rows, 0).int(), rows)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,rows,hidden", [(1, 70001, 1024), (9, 9001, 8192), (3000, 40003, 2048), (9000, 300000, 256), (64, 17, 4 << 20), (5, 20000, 4100)])
+def test_embedding_grad_of_large_tables(n, rows, hidden, dtype):
+    """Outputs much larger than what the tokens touch: every other row is cleared, and the last row is written."""
+    g = randn(n, hidden, dtype=BF16, seed=n)
+    for kind in ("skewed", "distinct"):
+        ids = spread(kind, n, rows, 0)
+        ids[0] = rows - 1
+        out = torch.full((rows, hidden), 7.0, dtype=dtype, device=DEV)
+        held = (ids >= 0) & (ids < rows)
+        V.embedding_grad(g, ids, rows, out=out)
+        at = ids[held].unique()
+        few = torch.searchsorted(at, ids)  # the same sums on a table of the touched rows alone
+        few = torch.where(held, few, -1)
+        assert torch.equal(out[at], V.embedding_grad(g, few, len(at), dtype=dtype))
+        out[at] = 0
+        assert not out.any()
+
+
 def test_embedding_grad_strides():
     ids = torch.randint(0, 30, (50, 4), generator=gen(3), device=DEV)
     big = randn(200, 300, dtype=BF16, seed=3)
