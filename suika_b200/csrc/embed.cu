@@ -470,7 +470,7 @@ int launch_sort(const SortArgs& a, int cluster, int grid, cudaStream_t st) {
   at[0].val.clusterDim.x = cluster;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1;
   return tcuda(cudaLaunchKernelEx(&cfg, sort_fill_kernel<R>, a), "rs_embed_grad: launch (sort)");
 }
 
