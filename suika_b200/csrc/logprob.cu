@@ -657,18 +657,20 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(BwdArgs a) {
     base = st.m;
     rest = logf(st.s);
   }
-  // with d = log p: gradient = p (wd d + w0), and g_lp more at the target
-  const float wd = -gh, w0 = -fmaf(gh, h, gp);
+  // with t = log2 p: gradient = wd (p t) + w0 p, and g_lp more at the target. p is multiplied first: where it is 0 the
+  // products are 0 whatever wd is, while wd t overflows for a masked logit's t (-1e37; |wd| > 34) and 0 * inf is NaN.
+  // Taking t instead of log p makes up for the third product (4096 rows of 32000 bf16: 88.1 us, 90.1 with log p).
+  const float wd = -gh * kLn2, w0 = -fmaf(gh, h, gp);
   const bool raised = moderate<T>(base);
-  const f32x2 minus = pair(-base, -base), less = pair(-rest, -rest), scale = pair(kLog2e, kLog2e), wd2 = pair(wd, wd), w02 = pair(w0, w0);
+  const f32x2 minus = pair(-base, -base), scale = pair(kLog2e, kLog2e), less = pair(-rest * kLog2e, -rest * kLog2e), wd2 = pair(wd, wd), w02 = pair(w0, w0);
   auto two = [&](float x, float y) {
-    f32x2 d = add2(add2(pair(x, y), minus), less);
-    const f32x2 p = exp2_pair(mul2(d, scale));
+    f32x2 t = fma2(add2(pair(x, y), minus), scale, less);
+    const f32x2 p = exp2_pair(t);
     if (!raised) {  // p is 0 below; -inf * 0 would be NaN
-      const float2 u = unpair(d);
-      d = pair(fmaxf(u.x, -1e4f), fmaxf(u.y, -1e4f));
+      const float2 u = unpair(t);
+      t = pair(fmaxf(u.x, -1e4f), fmaxf(u.y, -1e4f));
     }
-    return unpair(mul2(p, fma2(wd2, d, w02)));
+    return unpair(fma2(wd2, mul2(p, t), mul2(w02, p)));
   };
   const int per = kUnroll * kThreads;
   const uint4* src = reinterpret_cast<const uint4*>(z + head);
