@@ -106,7 +106,7 @@ typedef struct rs_program rs_program;
 
 const char* rs_last_error(void);
 /* 1.1 adds rs_copy_launch_noalloc, rs_act_plan and rs_act_resolve; 1.2 adds rs_copy_run_bounded;
- * 1.3 adds the training-step operators.
+ * 1.3 adds the training-step operators; 1.4 adds rs_token_logprobs_shard_grad.
  * The 1.0 entry points are unchanged. */
 int rs_version(int32_t* major, int32_t* minor);
 
@@ -510,7 +510,7 @@ typedef struct rs_logprob_opts {
   uint32_t dtype;
   int32_t wide_targets;   /* targets are int64, else int32 */
   int32_t top;            /* alternatives, 0..32 */
-  int32_t sharded;        /* gradient: a target outside the shard is another shard's, else it is no target */
+  int32_t sharded;        /* gradient: one of several shards; 0: a target outside [lo, lo + cols) is no target */
 } rs_logprob_opts;
 
 /* Per row: log probability of the target (0 where the target is in no shard), entropy, log-sum-exp, and the
@@ -528,10 +528,16 @@ int rs_token_merge(const float* records_dev, const int64_t* starts, int32_t n_sh
                    float* logprob_dev, float* entropy_dev, float* lse_dev, float* top_logprob_dev, int64_t* top_index_dev,
                    int32_t device, void* stream);
 /* d logits of sum(grad_logprob * logprob) + sum(grad_entropy * entropy) + sum(grad_lse * lse); grad_entropy_dev and
- * grad_lse_dev may be NULL, grad_dev may be the logits. lse and entropy are those of the whole vocabulary. A row of -inf alone has gradient 0. */
+ * grad_lse_dev may be NULL, grad_dev may be the logits. lse and entropy are those of the whole vocabulary. A row of -inf alone has gradient 0.
+ * With `sharded` every target of 0 or more is taken for one of the vocabulary's: where targets may lie past its end, or
+ * before its first index, use rs_token_logprobs_shard_grad, for which a target outside [vocab_first, vocab_end) is none. */
 int rs_token_logprobs_grad(const rs_logprob_opts* opts, const void* logits_dev, const void* targets_dev, const float* lse_dev,
                            const float* entropy_dev, const float* grad_logprob_dev, const float* grad_entropy_dev,
                            const float* grad_lse_dev, void* grad_dev, int64_t grad_stride, int32_t device, void* stream);
+int rs_token_logprobs_shard_grad(const rs_logprob_opts* opts, int64_t vocab_first, int64_t vocab_end, const void* logits_dev,
+                                 const void* targets_dev, const float* lse_dev, const float* entropy_dev, const float* grad_logprob_dev,
+                                 const float* grad_entropy_dev, const float* grad_lse_dev, void* grad_dev, int64_t grad_stride,
+                                 int32_t device, void* stream);
 
 #ifdef __cplusplus
 }

@@ -226,6 +226,7 @@ SIGNATURES = {
     "rs_token_record": (C.c_int, [C.POINTER(RsLogprobOpts), _P, _P, _P, C.c_int32, _P]),
     "rs_token_merge": (C.c_int, [_P, _P, C.c_int32, C.c_int64, C.c_int32, _P, _P, _P, _P, _P, C.c_int32, _P]),
     "rs_token_logprobs_grad": (C.c_int, [C.POINTER(RsLogprobOpts), _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, C.c_int32, _P]),
+    "rs_token_logprobs_shard_grad": (C.c_int, [C.POINTER(RsLogprobOpts), C.c_int64, C.c_int64, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, C.c_int32, _P]),
 }
 
 _lock = threading.Lock()

@@ -257,10 +257,11 @@ PyObject* token_record(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// token_logprobs_grad(logits, targets, lse, entropy, grad_logprob, grad_entropy, grad_lse, lo, sharded, out): None where allowed
+// token_logprobs_grad(logits, targets, lse, entropy, grad_logprob, grad_entropy, grad_lse, lo, sharded, out, first, end): None where
+// allowed; first and end are the whole vocabulary's where a shard's caller knows it
 PyObject* token_logprobs_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return entry([&]() -> PyObject* {
-    count_args("token_logprobs_grad", n, 10);
+    count_args("token_logprobs_grad", n, 12);
     const at::Tensor& logits = tensor(a[0], "logits");
     const Logits l(logits, tensor(a[1], "targets"), 0, integer(a[7]), truth(a[8]));
     if (a[5] != Py_None && a[3] == Py_None) value_error("a gradient of the entropy needs the entropy");
@@ -281,8 +282,12 @@ PyObject* token_logprobs_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
       value_error("out must have the logits' shape, type and device");
     const at::Tensor o = out.dim() == 2 ? out : out.view({-1, l.o.cols});
     if (o.stride(1) != 1 && l.o.cols > 1) value_error("out must have contiguous rows");
-    check(rs_token_logprobs_grad(&l.o, l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4], o.data_ptr(), o.stride(0),
-                                 logits.get_device(), stream_of(logits)));
+    if (a[10] == Py_None)
+      check(rs_token_logprobs_grad(&l.o, l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4], o.data_ptr(), o.stride(0),
+                                   logits.get_device(), stream_of(logits)));
+    else
+      check(rs_token_logprobs_shard_grad(&l.o, integer(a[10]), integer(a[11]), l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4],
+                                         o.data_ptr(), o.stride(0), logits.get_device(), stream_of(logits)));
     return THPVariable_Wrap(std::move(out));
   });
 }

@@ -602,8 +602,9 @@ struct BwdArgs {
   int64_t n, cols, stride;
   const void* targets;
   bool wide;
-  bool sharded;  // a target outside [lo, lo + cols) is another shard's; else it is none
+  bool sharded;  // one of several shards: a target outside [lo, lo + cols) may be another's
   int64_t lo;
+  int64_t first, end;  // the whole vocabulary: a target outside it is none
   const float* lse;
   const float* entropy;
   const float* grad_logprob;
@@ -624,11 +625,11 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(BwdArgs a) {
   const int first = (int)(blockIdx.x - row * a.ctas);
   const T* z = reinterpret_cast<const T*>(a.logits) + row * a.stride;
   T* out = reinterpret_cast<T*>(a.out) + row * a.out_stride;
-  const int64_t target = load_target(a.targets, a.wide, row) - a.lo;
+  const int64_t index = load_target(a.targets, a.wide, row), target = index - a.lo;
   const float lse = a.lse[row];
   const float h = a.entropy ? a.entropy[row] : 0.f, gh = a.grad_entropy ? a.grad_entropy[row] : 0.f;
   const int target_col = target >= 0 && target < a.cols ? (int)target : -1;
-  const bool ignored = a.sharded ? target + a.lo < 0 : target < 0 || target >= a.cols;
+  const bool ignored = index < a.first || index >= a.end;
   const float gl = ignored ? 0.f : a.grad_logprob[row];
   const float gz = a.grad_lse ? a.grad_lse[row] : 0.f, gp = gl - gz;
   const bool none = (gl == 0.f && gh == 0.f && gz == 0.f) || lse == -INFINITY;  // an empty row has no gradient
@@ -820,6 +821,66 @@ int forward(const char* what, const rs_logprob_opts* o, const void* logits, cons
   return launch_forward<__half>(a, sms, st);
 }
 
+// [first, end): the whole vocabulary, whose targets have a gradient.
+int backward(const char* what, const rs_logprob_opts* opts, int64_t first, int64_t end, const void* logits, const void* targets, const float* lse,
+             const float* entropy, const float* grad_logprob, const float* grad_entropy, const float* grad_lse, void* grad,
+             int64_t grad_stride, int32_t device, void* stream) {
+  int rc = check_opts(what, opts);
+  if (rc != RS_OK) return rc;
+  const rs_logprob_opts& o = *opts;
+  const std::string w(what);
+  if (o.n_rows == 0) return RS_OK;
+  const int b = dtype_bytes(o.dtype);
+  if (!logits || !targets || !lse || !grad_logprob || !grad || (grad_entropy && !entropy))
+    return tfail(RS_ERR_ARG, w + ": NULL address");
+  if ((uint64_t)logits % b || (uint64_t)grad % b || (uint64_t)targets % (o.wide_targets ? 8 : 4))
+    return tfail(RS_ERR_ARG, w + ": an address is not aligned to its elements");
+  if (o.n_rows > 1 && grad_stride < o.cols) return tfail(RS_ERR_ARG, w + ": the gradient's rows overlap");
+  BwdArgs a{};
+  a.logits = logits;
+  a.n = o.n_rows;
+  a.cols = o.cols;
+  a.stride = o.stride;
+  a.targets = targets;
+  a.wide = o.wide_targets != 0;
+  a.sharded = o.sharded != 0;
+  a.lo = o.lo;
+  a.first = first;
+  a.end = end;
+  a.lse = lse;
+  a.entropy = entropy;
+  a.grad_logprob = grad_logprob;
+  a.grad_entropy = grad_entropy;
+  a.grad_lse = grad_lse;
+  a.out = grad;
+  a.out_stride = grad_stride;
+  const int64_t per = (int64_t)kUnroll * kThreads * (16 / b);
+  const int64_t units = (o.cols + per - 1) / per;
+  if (units * o.n_rows > INT_MAX) return tfail(RS_ERR_CAPACITY, w + ": too many logits in one call");
+  a.units = (int)units;
+  // the output is the logits, lies beside them (columns of one buffer), or shares no memory with them
+  const uint64_t z0 = (uint64_t)logits, g0 = (uint64_t)grad;
+  const uint64_t z1 = z0 + ((uint64_t)(o.n_rows - 1) * o.stride + o.cols) * b, g1 = g0 + ((uint64_t)(o.n_rows - 1) * grad_stride + o.cols) * b;
+  const bool same = z0 == g0 && (o.stride == grad_stride || o.n_rows == 1);
+  if (!same && z0 < g1 && g0 < z1) {
+    const uint64_t pitch = (uint64_t)o.stride * b, width = (uint64_t)o.cols * b;
+    const uint64_t apart = pitch ? (g0 > z0 ? (g0 - z0) % pitch : (pitch - (z0 - g0) % pitch) % pitch) : 0;
+    if (o.stride != grad_stride || o.n_rows == 1 || apart < width || apart + width > pitch)
+      return tfail(RS_ERR_ARG, w + ": the gradient overlaps the logits without being them");
+  }
+  // up to four pieces per CTA, as long as sixteen CTAs per SM are left
+  const int64_t pieces = std::min<int64_t>(4, std::max<int64_t>(1, units * o.n_rows / ((int64_t)sm_count(device) * 16)));
+  a.ctas = same ? 1 : (int)((units + pieces - 1) / pieces);
+  DeviceGuard guard(device);
+  if (guard.err != cudaSuccess) return tcuda(guard.err, (w + ": cudaSetDevice").c_str());
+  cudaStream_t st = (cudaStream_t)stream;
+  const unsigned grid = (unsigned)(a.ctas * o.n_rows);
+  if (o.dtype == RS_F32) backward_kernel<float><<<grid, kThreads, 0, st>>>(a);
+  else if (o.dtype == RS_BF16) backward_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a);
+  else backward_kernel<__half><<<grid, kThreads, 0, st>>>(a);
+  return tcuda(cudaGetLastError(), (w + ": launch").c_str());
+}
+
 }  // namespace
 
 extern "C" {
@@ -873,57 +934,22 @@ int rs_token_logprobs_grad(const rs_logprob_opts* opts, const void* logits_dev, 
                            const float* entropy_dev, const float* grad_logprob_dev, const float* grad_entropy_dev,
                            const float* grad_lse_dev, void* grad_dev, int64_t grad_stride, int32_t device, void* stream) {
   return guarded("rs_token_logprobs_grad", [&]() -> int {
-    int rc = check_opts("rs_token_logprobs_grad", opts);
-    if (rc != RS_OK) return rc;
-    const rs_logprob_opts& o = *opts;
-    if (o.n_rows == 0) return RS_OK;
-    const int b = dtype_bytes(o.dtype);
-    if (!logits_dev || !targets_dev || !lse_dev || !grad_logprob_dev || !grad_dev || (grad_entropy_dev && !entropy_dev))
-      return tfail(RS_ERR_ARG, "rs_token_logprobs_grad: NULL address");
-    if ((uint64_t)logits_dev % b || (uint64_t)grad_dev % b || (uint64_t)targets_dev % (o.wide_targets ? 8 : 4))
-      return tfail(RS_ERR_ARG, "rs_token_logprobs_grad: an address is not aligned to its elements");
-    if (o.n_rows > 1 && grad_stride < o.cols) return tfail(RS_ERR_ARG, "rs_token_logprobs_grad: the gradient's rows overlap");
-    BwdArgs a{};
-    a.logits = logits_dev;
-    a.n = o.n_rows;
-    a.cols = o.cols;
-    a.stride = o.stride;
-    a.targets = targets_dev;
-    a.wide = o.wide_targets != 0;
-    a.sharded = o.sharded != 0;
-    a.lo = o.lo;
-    a.lse = lse_dev;
-    a.entropy = entropy_dev;
-    a.grad_logprob = grad_logprob_dev;
-    a.grad_entropy = grad_entropy_dev;
-    a.grad_lse = grad_lse_dev;
-    a.out = grad_dev;
-    a.out_stride = grad_stride;
-    const int64_t per = (int64_t)kUnroll * kThreads * (16 / b);
-    const int64_t units = (o.cols + per - 1) / per;
-    if (units * o.n_rows > INT_MAX) return tfail(RS_ERR_CAPACITY, "rs_token_logprobs_grad: too many logits in one call");
-    a.units = (int)units;
-    // the output is the logits, lies beside them (columns of one buffer), or shares no memory with them
-    const uint64_t z0 = (uint64_t)logits_dev, g0 = (uint64_t)grad_dev;
-    const uint64_t z1 = z0 + ((uint64_t)(o.n_rows - 1) * o.stride + o.cols) * b, g1 = g0 + ((uint64_t)(o.n_rows - 1) * grad_stride + o.cols) * b;
-    const bool same = z0 == g0 && (o.stride == grad_stride || o.n_rows == 1);
-    if (!same && z0 < g1 && g0 < z1) {
-      const uint64_t pitch = (uint64_t)o.stride * b, width = (uint64_t)o.cols * b;
-      const uint64_t apart = pitch ? (g0 > z0 ? (g0 - z0) % pitch : (pitch - (z0 - g0) % pitch) % pitch) : 0;
-      if (o.stride != grad_stride || o.n_rows == 1 || apart < width || apart + width > pitch)
-        return tfail(RS_ERR_ARG, "rs_token_logprobs_grad: the gradient overlaps the logits without being them");
-    }
-    // up to four pieces per CTA, as long as sixteen CTAs per SM are left
-    const int64_t pieces = std::min<int64_t>(4, std::max<int64_t>(1, units * o.n_rows / ((int64_t)sm_count(device) * 16)));
-    a.ctas = same ? 1 : (int)((units + pieces - 1) / pieces);
-    DeviceGuard guard(device);
-    if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_token_logprobs_grad: cudaSetDevice");
-    cudaStream_t st = (cudaStream_t)stream;
-    const unsigned grid = (unsigned)(a.ctas * o.n_rows);
-    if (o.dtype == RS_F32) backward_kernel<float><<<grid, kThreads, 0, st>>>(a);
-    else if (o.dtype == RS_BF16) backward_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a);
-    else backward_kernel<__half><<<grid, kThreads, 0, st>>>(a);
-    return tcuda(cudaGetLastError(), "rs_token_logprobs_grad: launch");
+    const bool whole = opts && !opts->sharded;
+    return backward("rs_token_logprobs_grad", opts, whole ? opts->lo : 0, whole ? opts->lo + opts->cols : INT64_MAX, logits_dev, targets_dev,
+                    lse_dev, entropy_dev, grad_logprob_dev, grad_entropy_dev, grad_lse_dev, grad_dev, grad_stride, device, stream);
+  });
+}
+
+int rs_token_logprobs_shard_grad(const rs_logprob_opts* opts, int64_t vocab_first, int64_t vocab_end, const void* logits_dev,
+                                 const void* targets_dev, const float* lse_dev, const float* entropy_dev, const float* grad_logprob_dev,
+                                 const float* grad_entropy_dev, const float* grad_lse_dev, void* grad_dev, int64_t grad_stride,
+                                 int32_t device, void* stream) {
+  return guarded("rs_token_logprobs_shard_grad", [&]() -> int {
+    if (!opts || !opts->sharded) return tfail(RS_ERR_ARG, "rs_token_logprobs_shard_grad: the options of a sharded gradient are taken");
+    if (opts->lo < vocab_first || opts->cols > vocab_end - opts->lo)
+      return tfail(RS_ERR_ARG, "rs_token_logprobs_shard_grad: the shard leaves the vocabulary");
+    return backward("rs_token_logprobs_shard_grad", opts, vocab_first, vocab_end, logits_dev, targets_dev, lse_dev, entropy_dev,
+                    grad_logprob_dev, grad_entropy_dev, grad_lse_dev, grad_dev, grad_stride, device, stream);
   });
 }
 

@@ -16,6 +16,7 @@ an eager graph of the same leaves lives. There is no CPU path.
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
@@ -133,22 +134,26 @@ def merge_token_records(records: torch.Tensor, starts: Sequence[int]) -> TokenLo
 
 
 def _forward(logits, targets, top, lo, group, starts):
+    """token_logprobs' five outputs and, over a group, the records of all shards."""
     if group is None:
-        return L.extension().token_logprobs(logits, targets, top, lo)
+        return L.extension().token_logprobs(logits, targets, top, lo), None
     world, cols = dist.get_world_size(group), logits.shape[-1]
     if starts is None:  # equal shards in rank order
         starts = [lo + (r - dist.get_rank(group)) * cols for r in range(world)]
     mine = L.extension().token_record(logits, targets, top, lo)
     everyone = torch.empty((world * mine.shape[0], mine.shape[1]), dtype=mine.dtype, device=mine.device)
     dist.all_gather_into_tensor(everyone, mine, group=group)
-    r = merge_token_records(everyone.view(world, *mine.shape), starts)
-    return tuple(None if t is None else t.reshape(*targets.shape, *t.shape[1:]) for t in r)
+    everyone = everyone.view(world, *mine.shape)
+    r = merge_token_records(everyone, starts)
+    return tuple(None if t is None else t.reshape(*targets.shape, *t.shape[1:]) for t in r), everyone
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top, lo, group, starts):
-        out = _forward(logits, targets, top, lo, group, starts)
+        out, records = _forward(logits, targets, top, lo, group, starts)
+        if records is not None:  # a target that no shard holds has no gradient on any
+            targets = targets.masked_fill((records[:, :, 3] == math.inf).all(0).view(targets.shape), -1)
         ctx.save_for_backward(logits, targets, out[2], out[1])
         ctx.lo, ctx.sharded = lo, group is not None
         if top:
@@ -180,16 +185,21 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
     shards). logprob, entropy and lse are differentiable with respect to logits."""
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top, lo, group, starts))
-    return TokenLogprobs(*_forward(logits, targets, top, lo, group, starts))
+    return TokenLogprobs(*_forward(logits, targets, top, lo, group, starts)[0])
 
 
 def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, entropy: Optional[torch.Tensor],
                         grad_logprob: torch.Tensor, grad_entropy: Optional[torch.Tensor] = None, *,
                         grad_lse: Optional[torch.Tensor] = None, lo: int = 0, sharded: bool = False,
-                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                        vocab: Optional[Tuple[int, int]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gradient of token_logprobs' logits, in their shape and type, from the gradients of logprob,
     entropy and lse (float32). lse and entropy are token_logprobs' own. `out` may be the logits themselves.
-    sharded=True: the logits are one of several shards, and a target outside it is another's; probabilities
-    then come from lse alone, whose 32 bits leave them off by |lse| 2^-24 (a whole row with |lse| over
-    1024 has its maximum and sum taken again)."""
-    return L.extension().token_logprobs_grad(logits, targets, lse, entropy, grad_logprob, grad_entropy, grad_lse, lo, sharded, out)
+    sharded=True: the logits are one of several shards; probabilities then come from lse alone, whose 32
+    bits leave them off by |lse| 2^-24 (a whole row with |lse| over 1024 has its maximum and sum taken
+    again). A target outside this shard is another's if it lies in `vocab`, the whole vocabulary's [first, end),
+    and none otherwise. Without `vocab` negative targets alone are none: give it where others may
+    lie outside the vocabulary (autograd through token_logprobs needs no telling)."""
+    if vocab is not None and not sharded:
+        raise ValueError("vocab is given with sharded=True")
+    first, end = vocab if vocab is not None else (None, None)
+    return L.extension().token_logprobs_grad(logits, targets, lse, entropy, grad_logprob, grad_entropy, grad_lse, lo, sharded, out, first, end)

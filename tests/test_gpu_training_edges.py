@@ -45,3 +45,76 @@ def test_masked_logits_have_no_gradient_whatever_the_entropys(dtype, cols, facto
         assert not got.isnan().any()
         assert (got[masked & ~hot] == 0).all()
         assert_close(torch.where(fits, got, 0), torch.where(fits, ref, 0), torch.where(fits, bound, 0))
+
+
+# ---- targets that no shard holds --------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cuts", [[0, 500], [0, 1, 30, 500], [0, 100, 200, 300, 400, 500]])
+def test_targets_outside_the_vocabulary_have_no_gradient_on_shards(dtype, cuts):
+    n, lo, end = 8, 1000, 1500
+    z = randn(n, 500, dtype=dtype, scale=2.0, seed=6)
+    t = torch.tensor([end, end + 7, lo - 1, 0, -1, -100, end - 1, lo], device=DEV)
+    gl, gh, gz = grads_of(n, 5)
+    recs = torch.stack([V.token_record(z[:, a:b], t, lo=lo + a) for a, b in zip(cuts, cuts[1:])])
+    r = V.merge_token_records(recs, [lo + a for a in cuts[:-1]])
+    assert not r.logprob[:6].any() and r.logprob[6:].all()
+    for tt in (t, t.int()):
+        for h, g in ((gh, gz), (None, None)):
+            ref, size = ref_grad(z, t, lo, gl, torch.zeros_like(gl) if h is None else h, torch.zeros_like(gl) if g is None else g)
+            got = torch.cat([V.token_logprobs_grad(z[:, a:b], tt, r.lse, r.entropy, gl, h, grad_lse=g, lo=lo + a, sharded=True, vocab=(lo, end))
+                             for a, b in zip(cuts, cuts[1:])], 1)
+            assert_close(got, ref, 400 * U * size + half(dtype) * ref.abs() + tiny(dtype))
+            if h is None:
+                assert not got[:6].any()
+
+
+def test_a_vocabulary_is_given_with_shards_only():
+    z, t, f = torch.zeros(3, 8, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV), torch.zeros(3, device=DEV)
+    with pytest.raises(ValueError, match="sharded"):
+        V.token_logprobs_grad(z, t, f, f, f, vocab=(0, 8))
+    for bad in ((4, 8), (0, 7), (8, 0)):
+        with pytest.raises(RuntimeError, match="vocabulary"):
+            V.token_logprobs_grad(z, t, f, f, f, sharded=True, vocab=bad)
+
+
+class Ranks:
+    """The collectives of suika_b200.vocab among ranks that run one after the other in this process."""
+
+    def __init__(self, monkeypatch):
+        monkeypatch.setattr(V, "dist", self)
+        self.rank, self.parts = 0, []
+
+    def get_world_size(self, group):
+        return self.world
+
+    def get_rank(self, group):
+        return self.rank
+
+    def all_gather_into_tensor(self, out, mine, group=None):
+        if len(self.parts) < self.world:
+            self.parts.append(mine.clone())
+            raise StopIteration
+        out.copy_(torch.cat(self.parts))
+
+    def run(self, world, call):
+        self.world, self.parts, done = world, [], []
+        for self.rank in range(world):
+            with pytest.raises(StopIteration):
+                call(self.rank)
+        for self.rank in range(world):
+            done.append(call(self.rank))
+        return done
+
+
+@pytest.mark.parametrize("cuts", [[0, 250, 500], [0, 100, 200, 300, 400, 500]])
+def test_targets_outside_the_vocabulary_over_a_group(monkeypatch, cuts):
+    ranks, n = Ranks(monkeypatch), 8
+    z = randn(n, 500, scale=2.0, seed=6)
+    t = torch.tensor([500, 507, 1 << 40, 499, -1, -100, 250, 0], device=DEV)
+    gl, gh, gz = grads_of(n, 5)
+    leaves = [z[:, a:b].clone().requires_grad_() for a, b in zip(cuts, cuts[1:])]
+    out = ranks.run(len(leaves), lambda r: V.token_logprobs(leaves[r], t, lo=cuts[r], group="ranks"))
+    for r in out:
+        ((r.logprob * gl).sum() + (r.entropy * gh).sum() + (r.lse * gz).sum()).backward()
+    ref, size = ref_grad(z, t, 0, gl, gh, gz)
+    assert_close(torch.cat([x.grad for x in leaves], 1), ref, 400 * U * size + 2.0 ** -126)
