@@ -179,7 +179,7 @@ struct FwdArgs {
   float* lse;
   float* top_value;
   int64_t* top_index;
-  float* record;   // [n][4 + 2 top]: m, S, A, target's logit (+inf: not here), values, local indices as bits
+  float* record;   // [n][4 + 2 top]: m, S, A, target's logit (+inf: not here; one that is +inf: NaN), values, local indices as bits
 };
 
 // What one row ends as. S = 0: every logit is -inf. Nothing is possible there: lse and every log
@@ -190,7 +190,7 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, int64_t row, const 
   const float log_s = logf(st.s);
   const float lse = empty ? -INFINITY : b + log_s;
   // target - m first: both are logits, their difference is small where it matters
-  const float lp = target == INFINITY && !isnan(lse) ? 0.f : empty ? -INFINITY : (target - b) - log_s;
+  const float lp = target == INFINITY ? 0.f : empty ? -INFINITY : (target - b) - log_s;
   a.logprob[row] = lp;
   a.entropy[row] = empty ? 0.f : fmaf(-kLn2, st.a / st.s, log_s);
   a.lse[row] = lse;
@@ -298,7 +298,10 @@ __global__ void __launch_bounds__(THREADS) forward_kernel(FwdArgs a, int cs) {
   float target = INFINITY;
   if (tid == 0) {
     const int64_t at = load_target(a.targets, a.wide, row) - a.lo;
-    if (at >= 0 && at < a.cols) target = to_f32<T>(sh.z[at]);
+    if (at >= 0 && at < a.cols) {
+      target = to_f32<T>(sh.z[at]);
+      if (target == INFINITY) target = NAN;  // +inf says that there is no target; in such a row the log probability is NaN
+    }
   }
   const float loose_z = tid < sh.loose ? to_f32<T>(sh.z[sh.loose_at(tid)]) : -INFINITY;
 

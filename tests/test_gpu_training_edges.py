@@ -118,3 +118,25 @@ def test_targets_outside_the_vocabulary_over_a_group(monkeypatch, cuts):
         ((r.logprob * gl).sum() + (r.entropy * gh).sum() + (r.lse * gz).sum()).backward()
     ref, size = ref_grad(z, t, 0, gl, gh, gz)
     assert_close(torch.cat([x.grad for x in leaves], 1), ref, 400 * U * size + 2.0 ** -126)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_targets_that_are_none_on_rows_of_nan_and_infinity(dtype):
+    """No target: log probability 0 and no gradient from it, whatever the row holds (the logits of padding are often NaN)."""
+    n, cols = 6, 700
+    z = randn(n, cols, dtype=dtype, seed=1)
+    z[0, 3], z[1, 4], z[2], z[3, 600], z[4, 699] = math.nan, math.inf, math.nan, math.inf, math.inf
+    none = torch.tensor([-1, -100, cols, 1 << 40, -1, -1], device=DEV)
+    r = V.token_logprobs(z, none)
+    assert (r.logprob == 0).all()
+    held = torch.tensor([5, 4, 5, 600, 5, 5], device=DEV)  # two of them the infinite logit itself
+    whole = V.token_logprobs(z, held)
+    assert whole.logprob[:5].isnan().all() and whole.logprob[5].isfinite()
+    gl = torch.ones(n, device=DEV)
+    assert not V.token_logprobs_grad(z, none, r.lse, r.entropy, gl).any()
+    cuts = [0, 100, 650, 700]
+    for t, want in ((none, r.logprob), (held, whole.logprob)):
+        recs = torch.stack([V.token_record(z[:, a:b], t, lo=a) for a, b in zip(cuts, cuts[1:])])
+        got = V.merge_token_records(recs, cuts[:-1])
+        assert torch.equal(got.logprob.isnan(), want.isnan())
+        assert_close(got.logprob, want, 700 * U * 12)
