@@ -105,19 +105,37 @@ def grad_sumsq(grads: Grads, counted: Optional[Counted] = None) -> torch.Tensor:
     return L.extension().grad_sumsq(_counted_parts(grads, counted), like)
 
 
+def _group_sumsq(grads: Grads, counted: Optional[Counted], group: Optional[dist.ProcessGroup], device: Optional[torch.device]) -> torch.Tensor:
+    """grad_sumsq summed over `group`; a rank without gradients brings 0 (on `device`), so that no other waits for it."""
+    if group is None:
+        return grad_sumsq(grads, counted)
+    if all(g is None for g in _listed(grads)):
+        sumsq = torch.zeros(1, dtype=torch.float64, device=device or torch.device("cuda", torch.cuda.current_device()))
+    else:
+        sumsq = grad_sumsq(grads, counted)
+    dist.all_reduce(sumsq, group=group)
+    return sumsq
+
+
+def _norm_of(sumsq: torch.Tensor) -> torch.Tensor:
+    return sumsq.sqrt().float().reshape(())
+
+
 def clip_grads(grads: Grads, max_norm: float, *, sumsq: Optional[torch.Tensor] = None, counted: Optional[Counted] = None,
                group: Optional[dist.ProcessGroup] = None) -> torch.Tensor:
     """Scale the gradients in place by min(1, max_norm / (norm + 1e-6)) and return the norm (float32, on
     the device; nothing is synchronised). The norm is that of grad_sumsq(grads, counted), summed over
     `group` if one is given, or sqrt(sumsq) if the caller has the global sum of squares already. All
     of every gradient is scaled, whether counted here or by another rank; gradients that share memory
-    are refused. A norm that is not finite reaches the gradients, as in torch.nn.utils.clip_grad_norm_."""
+    are refused. A norm that is not finite reaches the gradients, as in torch.nn.utils.clip_grad_norm_.
+    With `group` a rank may have no gradients (a frozen stage): it takes part in the sum, on the current device,
+    and gets the norm."""
     if not max_norm > 0:
         raise ValueError("max_norm must be positive")
     if sumsq is None and (counted is not None or group is not None):
-        sumsq = grad_sumsq(grads, counted)
-        if group is not None:
-            dist.all_reduce(sumsq, group=group)
+        sumsq = _group_sumsq(grads, counted, group, None)
+    if group is not None and all(g is None for g in _listed(grads)):
+        return _norm_of(sumsq)
     return L.extension().grad_clip(_listed(grads), max_norm, sumsq)
 
 
@@ -199,14 +217,15 @@ class ShardAdamW:
     def step(self, grads: Dict[str, torch.Tensor], *, sumsq: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """One update from {name: gradient}; names without a gradient (missing or None) stay as they are.
         Returns the norm before clipping (float32, on the device), or None without max_norm. `sumsq`:
-        the global sum of squares, if the caller has it already."""
+        the global sum of squares, if the caller has it already. With a group, or a given sumsq, there may be
+        no gradient at all: the rank takes part in the sum and nothing is updated."""
         gs = [grads.get(n) for n in self.names]
         if len(grads) > len(gs) or any(g is None for g in gs):
             extra = [n for n, g in grads.items() if g is not None and n not in self.state]
             if extra:
                 raise AssertionError(f"gradients of names that the state does not hold: {extra[:3]}")
         if self.max_norm is not None and sumsq is None and (self.counted is not None or self.group is not None):
-            sumsq = grad_sumsq({n: g for n, g in zip(self.names, gs)}, self.counted)
-            if self.group is not None:
-                dist.all_reduce(sumsq, group=self.group)
+            sumsq = _group_sumsq(dict(zip(self.names, gs)), self.counted, self.group, self.device)
+        if (self.group is not None or sumsq is not None) and all(g is None for g in gs):
+            return _norm_of(sumsq) if self.max_norm is not None else None
         return L.extension().adamw_step(*self._fields, self._decays, gs, self.lr, *self.betas, self.eps, self.weight_decay, self.max_norm, sumsq)

@@ -1,12 +1,19 @@
 """The training-step operators at the edges of what their documentation allows, on a B200, against a plain
 computation in 64 bits where numbers are compared."""
+import datetime
+import json
 import math
+import os
+import tempfile
+import traceback
 
 import pytest
 import torch
 
+from suika_b200 import optimizer as OPT
 from suika_b200 import vocab as V
-from tests.test_gpu_training import (DEV, TYPES, U, assert_close, grads_of, half, randn, ref_grad, ref_log_p, stat_rel, tiny)
+from tests.test_gpu_training import (BF16, DEV, F32, HYPER, TYPES, U, assert_close, clone_state, grads_of, half, make_state, randn,
+                                     ref_grad, ref_log_p, stat_rel, tiny)
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +147,69 @@ def test_targets_that_are_none_on_rows_of_nan_and_infinity(dtype):
         got = V.merge_token_records(recs, cuts[:-1])
         assert torch.equal(got.logprob.isnan(), want.isnan())
         assert_close(got.logprob, want, 700 * U * 12)
+
+
+# ---- a rank without gradients -----------------------------------------------------------------
+def test_a_rank_without_gradients_takes_part_in_the_sum(monkeypatch):
+    sums = []
+
+    class Dist:
+        @staticmethod
+        def all_reduce(t, group=None):
+            sums.append((t.clone(), group))
+            t.add_(9.0)
+    monkeypatch.setattr(OPT, "dist", Dist)
+    for grads in ({}, {"a": None}, []):
+        norm = OPT.clip_grads(grads, 1.0, group="ranks")
+        assert norm.shape == () and norm.dtype == F32 and float(norm) == 3.0
+    assert float(OPT.clip_grads({"a": None}, 1.0, counted={"a": [(0, 4)]}, group="ranks")) == 3.0
+    state = make_state([10], BF16, F32, True)
+    old = clone_state(state)
+    opt = OPT.ShardAdamW(state, max_norm=1.0, group="ranks", **HYPER)
+    for grads in ({}, {"t0": None}):
+        norm = opt.step(grads)
+        assert norm.shape == () and norm.dtype == F32 and float(norm) == 3.0
+    assert len(sums) == 6 and all(float(s) == 0.0 and s.dtype == torch.float64 and s.is_cuda and g == "ranks" for s, g in sums)
+    given = torch.full((1,), 16.0, dtype=torch.float64, device=DEV)
+    assert float(opt.step({}, sumsq=given)) == 4.0 and float(OPT.clip_grads([], 1.0, sumsq=given, group="ranks")) == 4.0 and len(sums) == 6
+    assert OPT.ShardAdamW(state, group="ranks", **HYPER).step({}) is None
+    assert all(torch.equal(state[n][s], old[n][s]) for n in old for s in old[n])
+    with pytest.raises(ValueError, match="no gradients"):  # alone there is nothing to take part in
+        OPT.clip_grads({"a": None}, 1.0)
+    with pytest.raises(ValueError, match="no gradients"):
+        OPT.ShardAdamW(state, max_norm=1.0, **HYPER).step({})
+
+
+def _empty_rank_worker(rank, world, port, outdir):
+    res = {}
+    try:
+        os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), NCCL_NVLS_ENABLE="0")
+        import torch.distributed as dist
+        from tests.helpers import rank_device
+        dev, backend = rank_device(rank, world)
+        torch.cuda.set_device(dev)
+        dist.init_process_group(backend, rank=rank, world_size=world, timeout=datetime.timedelta(seconds=60))
+        grads = {"a": torch.full((4,), 2.0, device=dev)} if rank == 0 else {"a": None}
+        res["clip"] = float(OPT.clip_grads(grads, 1.0, group=dist.group.WORLD))
+        state = {"a": {"param": torch.ones(4, device=dev), "exp_avg": torch.zeros(4, device=dev), "exp_avg_sq": torch.zeros(4, device=dev),
+                       "step": torch.tensor(0.0, device=dev)}}
+        opt = OPT.ShardAdamW(state, max_norm=1.0, group=dist.group.WORLD)
+        res["norm"] = float(opt.step({"a": torch.full((4,), 3.0, device=dev)} if rank == 0 else {}))
+        res["step"] = float(state["a"]["step"])
+        dist.barrier()
+        dist.destroy_process_group()
+    except Exception:
+        res["error"] = traceback.format_exc()
+    with open(os.path.join(outdir, f"rank{rank}.json"), "w") as f:
+        json.dump(res, f)
+
+
+def test_two_ranks_one_of_them_without_gradients():
+    """One process per rank (gloo where they share a GPU); no kernel waits on the other rank."""
+    import torch.multiprocessing as mp
+    with tempfile.TemporaryDirectory() as d:
+        mp.spawn(_empty_rank_worker, args=(2, 29790, d), nprocs=2, join=True)
+        results = [json.load(open(os.path.join(d, f"rank{r}.json"))) for r in range(2)]
+    for rank, r in enumerate(results):
+        assert "error" not in r, r.get("error")
+        assert r == {"clip": 4.0, "norm": 6.0, "step": 1.0 - rank}
