@@ -106,7 +106,7 @@ typedef struct rs_program rs_program;
 
 const char* rs_last_error(void);
 /* 1.1 adds rs_copy_launch_noalloc, rs_act_plan and rs_act_resolve; 1.2 adds rs_copy_run_bounded;
- * 1.3 adds the training-step operators; 1.4 adds rs_token_logprobs_shard_grad.
+ * 1.3 adds the training-step operators; 1.4 adds rs_token_logprobs_shard_grad and rs_token_record_at.
  * The 1.0 entry points are unchanged. */
 int rs_version(int32_t* major, int32_t* minor);
 
@@ -521,9 +521,12 @@ int rs_token_logprobs(const rs_logprob_opts* opts, const void* logits_dev, const
                       void* stream);
 /* The same for one shard of several: a record of 4 + 2 top floats per row, and the join of all shards' records,
  * [n_shards][n_rows][4 + 2 top] with shards in ascending order of their first index, starts[s] (host
- * memory; at most 64 shards). */
+ * memory; at most 64 shards). rs_token_record_at adds index_base to the record's indices: with the shard's first
+ * index there, all starts are 0 and a rank need not know the others'. */
 int rs_token_record(const rs_logprob_opts* opts, const void* logits_dev, const void* targets_dev, float* record_dev,
                     int32_t device, void* stream);
+int rs_token_record_at(const rs_logprob_opts* opts, int64_t index_base, const void* logits_dev, const void* targets_dev, float* record_dev,
+                       int32_t device, void* stream);
 int rs_token_merge(const float* records_dev, const int64_t* starts, int32_t n_shards, int64_t n_rows, int32_t top,
                    float* logprob_dev, float* entropy_dev, float* lse_dev, float* top_logprob_dev, int64_t* top_index_dev,
                    int32_t device, void* stream);

@@ -224,6 +224,7 @@ SIGNATURES = {
     "rs_embed_grad": (C.c_int, [C.POINTER(RsEmbedOpts), _P, _P, _P, _P, C.c_uint64, C.c_int32, _P]),
     "rs_token_logprobs": (C.c_int, [C.POINTER(RsLogprobOpts), _P, _P, _P, _P, _P, _P, _P, C.c_int32, _P]),
     "rs_token_record": (C.c_int, [C.POINTER(RsLogprobOpts), _P, _P, _P, C.c_int32, _P]),
+    "rs_token_record_at": (C.c_int, [C.POINTER(RsLogprobOpts), C.c_int64, _P, _P, _P, C.c_int32, _P]),
     "rs_token_merge": (C.c_int, [_P, _P, C.c_int32, C.c_int64, C.c_int32, _P, _P, _P, _P, _P, C.c_int32, _P]),
     "rs_token_logprobs_grad": (C.c_int, [C.POINTER(RsLogprobOpts), _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, C.c_int32, _P]),
     "rs_token_logprobs_shard_grad": (C.c_int, [C.POINTER(RsLogprobOpts), C.c_int64, C.c_int64, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, C.c_int32, _P]),

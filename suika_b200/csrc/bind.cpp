@@ -244,15 +244,15 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// token_record(logits, targets, top, lo) -> [rows, 4 + 2 top]
+// token_record(logits, targets, top, lo, index_base) -> [rows, 4 + 2 top]
 PyObject* token_record(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return entry([&]() -> PyObject* {
-    count_args("token_record", n, 4);
+    count_args("token_record", n, 5);
     const int64_t top = top_of(a[2]);
     const at::Tensor& logits = tensor(a[0], "logits");
     const Logits l(logits, tensor(a[1], "targets"), top, integer(a[3]), true);
     at::Tensor out = at::empty({l.o.n_rows, 4 + 2 * top}, logits.options().dtype(at::kFloat));
-    check(rs_token_record(&l.o, l.z.data_ptr(), l.targets.data_ptr(), out.data_ptr<float>(), logits.get_device(), stream_of(logits)));
+    check(rs_token_record_at(&l.o, integer(a[4]), l.z.data_ptr(), l.targets.data_ptr(), out.data_ptr<float>(), logits.get_device(), stream_of(logits)));
     return THPVariable_Wrap(std::move(out));
   });
 }

@@ -173,13 +173,14 @@ struct FwdArgs {
   bool wide;
   int64_t lo;
   int top;
+  int index_base;  // added to the indices of a record
   int per_note;    // iterations that share a note
   float* logprob;  // null: write records
   float* entropy;
   float* lse;
   float* top_value;
   int64_t* top_index;
-  float* record;   // [n][4 + 2 top]: m, S, A, target's logit (+inf: not here; one that is +inf: NaN), values, local indices as bits
+  float* record;   // [n][4 + 2 top]: m, S, A, target's logit (+inf: not here; one that is +inf: NaN), values, indices as bits
 };
 
 // What one row ends as. S = 0: every logit is -inf. Nothing is possible there: lse and every log
@@ -546,7 +547,7 @@ __global__ void __launch_bounds__(THREADS) forward_kernel(FwdArgs a, int cs) {
     if (a.record) {
       float* r = a.record + row * (4 + 2 * k) + 4;
       r[tid] = v;
-      r[k + tid] = __int_as_float(i);
+      r[k + tid] = __int_as_float(none ? -1 : a.index_base + i);
     } else {
       a.top_value[row * k + tid] = log_prob_of(v, t);
       a.top_index[row * k + tid] = none ? -1 : a.lo + i;
@@ -791,7 +792,7 @@ int launch_forward(const FwdArgs& a, int sms, cudaStream_t st) {
 }
 
 int forward(const char* what, const rs_logprob_opts* o, const void* logits, const void* targets, float* logprob, float* entropy, float* lse,
-            float* top_value, int64_t* top_index, float* record, int32_t device, void* stream) {
+            float* top_value, int64_t* top_index, float* record, int index_base, int32_t device, void* stream) {
   int rc = check_opts(what, o);
   if (rc != RS_OK) return rc;
   if (o->n_rows == 0) return RS_OK;
@@ -817,6 +818,7 @@ int forward(const char* what, const rs_logprob_opts* o, const void* logits, cons
   a.top_value = top_value;
   a.top_index = top_index;
   a.record = record;
+  a.index_base = index_base;
   const int sms = sm_count(device);
   cudaStream_t st = (cudaStream_t)stream;
   if (o->dtype == RS_F32) return launch_forward<float>(a, sms, st);
@@ -892,7 +894,7 @@ int rs_token_logprobs(const rs_logprob_opts* opts, const void* logits_dev, const
                       float* lse_dev, float* top_logprob_dev, int64_t* top_index_dev, int32_t device, void* stream) {
   return guarded("rs_token_logprobs", [&]() -> int {
     return forward("rs_token_logprobs", opts, logits_dev, targets_dev, logprob_dev, entropy_dev, lse_dev, top_logprob_dev, top_index_dev,
-                   nullptr, device, stream);
+                   nullptr, 0, device, stream);
   });
 }
 
@@ -900,7 +902,19 @@ int rs_token_record(const rs_logprob_opts* opts, const void* logits_dev, const v
                     void* stream) {
   return guarded("rs_token_record", [&]() -> int {
     if (opts && opts->n_rows > 0 && !record_dev) return tfail(RS_ERR_ARG, "rs_token_record: NULL record");
-    return forward("rs_token_record", opts, logits_dev, targets_dev, nullptr, nullptr, nullptr, nullptr, nullptr, record_dev, device, stream);
+    return forward("rs_token_record", opts, logits_dev, targets_dev, nullptr, nullptr, nullptr, nullptr, nullptr, record_dev, 0, device, stream);
+  });
+}
+
+int rs_token_record_at(const rs_logprob_opts* opts, int64_t index_base, const void* logits_dev, const void* targets_dev, float* record_dev,
+                       int32_t device, void* stream) {
+  return guarded("rs_token_record_at", [&]() -> int {
+    if (opts && opts->n_rows > 0 && !record_dev) return tfail(RS_ERR_ARG, "rs_token_record_at: NULL record");
+    if (index_base < 0) return tfail(RS_ERR_ARG, "rs_token_record_at: a negative index");
+    if (opts && (index_base > INT_MAX || opts->cols > INT_MAX - index_base))
+      return tfail(RS_ERR_CAPACITY, "rs_token_record_at: indices past 31 bits");
+    return forward("rs_token_record_at", opts, logits_dev, targets_dev, nullptr, nullptr, nullptr, nullptr, nullptr, record_dev, (int)index_base,
+                   device, stream);
   });
 }
 

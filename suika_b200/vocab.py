@@ -110,7 +110,7 @@ class TokenLogprobs(NamedTuple):
 
 def token_record(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0, lo: int = 0) -> torch.Tensor:
     """One vocabulary shard's part of token_logprobs: float32 [rows, 4 + 2 top], for merge_token_records."""
-    return L.extension().token_record(logits, targets, top, lo)
+    return L.extension().token_record(logits, targets, top, lo, 0)
 
 
 def merge_token_records(records: torch.Tensor, starts: Sequence[int]) -> TokenLogprobs:
@@ -137,14 +137,13 @@ def _forward(logits, targets, top, lo, group, starts):
     """token_logprobs' five outputs and, over a group, the records of all shards."""
     if group is None:
         return L.extension().token_logprobs(logits, targets, top, lo), None
-    world, cols = dist.get_world_size(group), logits.shape[-1]
-    if starts is None:  # equal shards in rank order
-        starts = [lo + (r - dist.get_rank(group)) * cols for r in range(world)]
-    mine = L.extension().token_record(logits, targets, top, lo)
+    world = dist.get_world_size(group)
+    # without starts a rank knows its own place alone: its record holds indices of the whole vocabulary
+    mine = L.extension().token_record(logits, targets, top, lo, lo if starts is None else 0)
     everyone = torch.empty((world * mine.shape[0], mine.shape[1]), dtype=mine.dtype, device=mine.device)
     dist.all_gather_into_tensor(everyone, mine, group=group)
     everyone = everyone.view(world, *mine.shape)
-    r = merge_token_records(everyone, starts)
+    r = merge_token_records(everyone, [0] * world if starts is None else starts)
     return tuple(None if t is None else t.reshape(*targets.shape, *t.shape[1:]) for t in r), everyone
 
 
@@ -180,9 +179,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
     vocabulary of fewer than `top` tokens fills up with index -1 and -inf. Logits of -inf (a mask)
     have probability 0; a row of nothing else has lse and log probabilities -inf, entropy 0 and gradient 0.
 
-    With `group`, the ranks of a TP group that hold the vocabulary's shards in rank order, the result is
-    that of the whole vocabulary on every rank; `starts`: the shards' first indices (default: equal
-    shards). logprob, entropy and lse are differentiable with respect to logits."""
+    With `group`, the ranks of a TP group that hold the vocabulary's shards in rank order (of any sizes), the
+    result is that of the whole vocabulary on every rank; `starts`: the shards' first indices, needed only past
+    31 bits. logprob, entropy and lse are differentiable with respect to logits."""
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top, lo, group, starts))
     return TokenLogprobs(*_forward(logits, targets, top, lo, group, starts)[0])

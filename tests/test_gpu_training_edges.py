@@ -12,7 +12,7 @@ import torch
 
 from suika_b200 import optimizer as OPT
 from suika_b200 import vocab as V
-from tests.test_gpu_training import (BF16, DEV, F32, HYPER, TYPES, U, assert_close, clone_state, grads_of, half, make_state, randn,
+from tests.test_gpu_training import (BF16, DEV, F32, HYPER, TYPES, U, assert_close, clone_state, gen, grads_of, half, make_state, randn,
                                      ref_grad, ref_log_p, stat_rel, tiny)
 
 pytestmark = pytest.mark.gpu
@@ -213,3 +213,20 @@ def test_two_ranks_one_of_them_without_gradients():
     for rank, r in enumerate(results):
         assert "error" not in r, r.get("error")
         assert r == {"clip": 4.0, "norm": 6.0, "step": 1.0 - rank}
+
+
+# ---- shards of unequal size -------------------------------------------------------------------
+@pytest.mark.parametrize("cuts", [[0, 1, 30, 500], [0, 300, 500], [7, 207, 407, 500], [0, 250, 500]])
+@pytest.mark.parametrize("top", [0, 1, 32])
+def test_unequal_shards_over_a_group_find_their_places(monkeypatch, cuts, top):
+    ranks, n, z = Ranks(monkeypatch), 9, randn(9, 500, dtype=BF16, scale=2.0, seed=2)
+    z[1], z[2, 40:] = 1.0, -math.inf
+    z = z[:, :cuts[-1] - cuts[0]]
+    t = cuts[0] + torch.randint(0, z.shape[1], (n,), generator=gen(1), device=DEV)
+    whole = V.token_logprobs(z, t, top=top, lo=cuts[0])
+    parts = [z[:, a - cuts[0]:b - cuts[0]] for a, b in zip(cuts, cuts[1:])]
+    for starts in (None, cuts[:-1]):
+        for r in ranks.run(len(parts), lambda i: V.token_logprobs(parts[i], t, top=top, lo=cuts[i], group="ranks", starts=starts)):
+            assert_close(r.logprob, whole.logprob, 500 * U * 12)
+            if top:
+                assert torch.equal(r.top_index, whole.top_index)

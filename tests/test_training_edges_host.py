@@ -17,3 +17,14 @@ def test_shard_gradient_entry_checks_the_vocabulary():
     assert call(0, 24, sharded=0) == L.RS_ERR_ARG and b"sharded" in lib.rs_last_error()
     assert call(16, 24) == L.RS_ERR_ARG and b"NULL" in lib.rs_last_error()  # the rest as in the entry without a range
     assert lib.rs_token_logprobs_shard_grad(None, 0, 8, *[FAKE] * 8, 8, 0, None) == L.RS_ERR_ARG
+
+
+def test_record_entry_checks_its_index_base():
+    lib = L.load()
+
+    def call(base, cols=8):
+        return lib.rs_token_record_at(ctypes.byref(L.RsLogprobOpts(4, cols, 8, 0, 0, 1, 2, 1)), base, FAKE, None, FAKE, 0, None)
+    assert call(-1) == L.RS_ERR_ARG and b"negative" in lib.rs_last_error()
+    for base in ((1 << 31) - 8, 1 << 31, (1 << 63) - 1):
+        assert call(base) == L.RS_ERR_CAPACITY, base
+    assert call((1 << 31) - 9) == L.RS_ERR_ARG and b"NULL" in lib.rs_last_error()
