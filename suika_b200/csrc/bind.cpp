@@ -100,6 +100,11 @@ at::Tensor index_tensor(const at::Tensor& t, const at::Tensor& with, const char*
   return t.contiguous();
 }
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+// A tensor that a kernel wrote in place counts as written for autograd, as after torch's own in-place operators: a
+// backward pass over what it held before is then an error. (Inference tensors keep no versions.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 std::string shape_of(at::IntArrayRef s) {
   std::string r = "[";
   for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
@@ -182,6 +187,7 @@ PyObject* embed_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check(rs_embed_grad_workspace_bytes(&o, device, &bytes));
     const at::Tensor workspace = at::empty({(int64_t)bytes}, grad_out.options().dtype(at::kByte));
     check(rs_embed_grad(&o, ids.data_ptr(), g.data_ptr(), out.data_ptr(), workspace.data_ptr(), bytes, device, stream_of(grad_out)));
+    if (a[6] != Py_None) written(out);
     return THPVariable_Wrap(std::move(out));
   });
 }
@@ -288,6 +294,7 @@ PyObject* token_logprobs_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     else
       check(rs_token_logprobs_shard_grad(&l.o, integer(a[10]), integer(a[11]), l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4],
                                          o.data_ptr(), o.stride(0), logits.get_device(), stream_of(logits)));
+    if (a[9] != Py_None) written(out);
     return THPVariable_Wrap(std::move(out));
   });
 }
@@ -357,6 +364,7 @@ PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
     check(rs_grad_clip(s.data(), (int64_t)s.size(), given_sumsq(sumsq, first), max_norm, norm.data_ptr<float>(), first.get_device(),
                        stream_of(first)));
+    for (const at::Tensor* t : ts) written(*t);
     return THPVariable_Wrap(std::move(norm));
   });
 }
@@ -421,6 +429,11 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor workspace = at::empty({(int64_t)bytes}, first.options().dtype(at::kByte));
     check(rs_adamw_step(t.data(), (int64_t)t.size(), &o, sumsq.defined() ? sumsq.data_ptr<double>() : nullptr, clip ? norm.data_ptr<float>() : nullptr,
                         workspace.data_ptr(), bytes, first.get_device(), stream_of(first)));
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[6]); ++i) {
+      if (PyList_GET_ITEM(a[6], i) == Py_None) continue;
+      for (int list = 0; list < 5; ++list)
+        if (PyList_GET_ITEM(a[list], i) != Py_None) written(tensor(PyList_GET_ITEM(a[list], i), "a sub-field"));
+    }
     return clip ? THPVariable_Wrap(std::move(norm)) : Py_NewRef(Py_None);
   });
 }

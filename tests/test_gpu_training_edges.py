@@ -230,3 +230,47 @@ def test_unequal_shards_over_a_group_find_their_places(monkeypatch, cuts, top):
             assert_close(r.logprob, whole.logprob, 500 * U * 12)
             if top:
                 assert torch.equal(r.top_index, whole.top_index)
+
+
+# ---- tensors that autograd follows --------------------------------------------------------------
+def test_what_is_written_in_place_counts_as_written():
+    state = make_state([100, 7], BF16, F32, True)
+    grads = {n: randn(e["param"].numel(), dtype=BF16, seed=1) for n, e in state.items()}
+    before = {n: {s: t._version for s, t in e.items()} for n, e in state.items()}
+    opt = OPT.ShardAdamW(state, max_norm=1.0, **HYPER)
+    opt.step({"t0": grads["t0"]})
+    assert all(t._version > before["t0"][s] for s, t in state["t0"].items())
+    assert all(t._version == before["t1"][s] for s, t in state["t1"].items())
+    v = grads["t0"]._version
+    OPT.clip_grads(grads, 1e-3)
+    assert grads["t0"]._version > v
+    ids, g = torch.arange(3, device=DEV), randn(3, 6, seed=2)
+    out = torch.zeros(4, 6, device=DEV)
+    v = out._version
+    V.embedding_grad(g, ids, 4, out=out)
+    assert out._version > v
+    z, t = randn(3, 8, seed=1), torch.zeros(3, dtype=torch.int64, device=DEV)
+    r = V.token_logprobs(z, t)
+    v = z._version
+    V.token_logprobs_grad(z, t, r.lse, r.entropy, r.lse, out=z)
+    assert z._version > v
+
+
+def test_a_backward_pass_over_what_was_written_is_an_error():
+    state = make_state([12], F32, F32, False)
+    w = state["t0"]["param"].requires_grad_()
+    y = (w * w).sum()
+    OPT.ShardAdamW(state, **HYPER).step({"t0": randn(12, seed=1)})
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    z = randn(3, 8, seed=1).requires_grad_()
+    t = torch.zeros(3, dtype=torch.int64, device=DEV)
+    r = V.token_logprobs(z, t)
+    V.token_logprobs_grad(z.detach(), t, r.lse.detach(), r.entropy.detach(), r.lse.detach(), out=z.detach())
+    with pytest.raises(RuntimeError, match="inplace"):
+        r.logprob.sum().backward()
+    with torch.inference_mode():  # no versions are kept there
+        s = make_state([12], F32, F32, False)
+        g = {"t0": randn(12, seed=1)}
+    OPT.ShardAdamW(s, max_norm=1.0, **HYPER).step(g)
+    OPT.clip_grads(g, 1.0)
