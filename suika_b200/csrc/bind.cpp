@@ -58,7 +58,10 @@ void count_args(const char* what, Py_ssize_t got, Py_ssize_t want) {
 }
 const at::Tensor& tensor(PyObject* o, const char* what) {
   if (!THPVariable_Check(o)) throw Raise{PyExc_TypeError, std::string(what) + " must be a tensor"};
-  return THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  // a kernel would drop the tangent without a word (levels of forward-mode AD do not nest: 0 is the only one)
+  if (t._fw_grad(0).defined()) value_error(std::string(what) + " with a forward-mode tangent: reverse mode alone is there");
+  return t;
 }
 double number(PyObject* o) {
   const double v = PyFloat_AsDouble(o);

@@ -9,9 +9,9 @@ on the vocabulary rows [lo, lo + rows) that its TensorMeta gives it (shard_range
   - token_logprobs / token_logprobs_grad: log probability of given tokens, entropy, log-sum-exp and
     top alternatives from one pass over the logits; over several shards (`group`) each rank sends a
     record of 4 + 2 top floats per row, not its logits.
-embedding and token_logprobs are differentiable (torch.autograd). Every call is stream-ordered on the
-current stream of the tensors' device and can be captured into a CUDA graph. To capture a backward
-pass, call embedding_grad and token_logprobs_grad: torch's autograd engine cannot be captured while
+embedding and token_logprobs are differentiable (torch.autograd, reverse mode). Every call is
+stream-ordered on the current stream of the tensors' device and can be captured into a CUDA graph. To
+capture a backward pass, call embedding_grad and token_logprobs_grad: torch's autograd engine cannot be captured while
 an eager graph of the same leaves lives. There is no CPU path.
 """
 from __future__ import annotations
@@ -22,6 +22,7 @@ from typing import NamedTuple, Optional, Sequence, Tuple
 import numpy as np
 import torch
 import torch.distributed as dist
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -119,6 +120,8 @@ def merge_token_records(records: torch.Tensor, starts: Sequence[int]) -> TokenLo
     dev = records.device
     if dev.type != "cuda":
         raise ValueError("records must be a CUDA tensor")
+    if forward_ad.unpack_dual(records).tangent is not None:
+        raise ValueError("records with a forward-mode tangent: reverse mode alone is there")
     if records.dim() != 3 or records.dtype != torch.float32 or not records.is_contiguous() or records.shape[2] < 4 or records.shape[2] % 2:
         raise ValueError("records must be a contiguous float32 [shards, rows, 4 + 2 top]")
     shards, n, words = records.shape

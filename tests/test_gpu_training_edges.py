@@ -274,3 +274,18 @@ def test_a_backward_pass_over_what_was_written_is_an_error():
         g = {"t0": randn(12, seed=1)}
     OPT.ShardAdamW(s, max_norm=1.0, **HYPER).step(g)
     OPT.clip_grads(g, 1.0)
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwad
+    w, z = randn(5, 6, seed=1), randn(3, 8, seed=2)
+    ids, t, f = torch.arange(3, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV), torch.zeros(3, device=DEV)
+    with fwad.dual_level():
+        dw, dz = fwad.make_dual(w, torch.ones_like(w)), fwad.make_dual(z, torch.ones_like(z))
+        rec = fwad.make_dual(torch.zeros(1, 3, 4, device=DEV), torch.ones(1, 3, 4, device=DEV))
+        for call in (lambda: V.embedding(ids, dw), lambda: V.embedding_grad(dw[:3], ids, 5), lambda: V.token_logprobs(dz, t, top=2),
+                     lambda: V.token_record(dz, t), lambda: V.token_logprobs_grad(dz, t, f, f, f), lambda: OPT.grad_sumsq([dw]),
+                     lambda: OPT.clip_grads([dw], 1.0), lambda: V.merge_token_records(rec, [0])):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        V.embedding(ids, w), V.token_logprobs(z, t)  # tensors without a tangent
