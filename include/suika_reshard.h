@@ -496,7 +496,7 @@ typedef struct rs_embed_opts {
 int rs_embed_lookup(const rs_embed_opts* opts, const void* ids_dev, const void* weight_dev, void* out_dev, int32_t device,
                     void* stream);
 /* grad[r] (+)= scale * sum of grad_out[i] over the tokens whose id is lo + r, in 32 bits; grad is contiguous
- * [rows, hidden]. At most 65536 tokens (RS_ERR_CAPACITY). */
+ * [rows, hidden] and shares no memory with grad_out. At most 65536 tokens (RS_ERR_CAPACITY). */
 int rs_embed_grad_workspace_bytes(const rs_embed_opts* opts, int32_t device, uint64_t* bytes);
 int rs_embed_grad(const rs_embed_opts* opts, const void* ids_dev, const void* grad_out_dev, void* grad_dev,
                   void* workspace_dev, uint64_t workspace_bytes, int32_t device, void* stream);

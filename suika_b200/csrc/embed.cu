@@ -433,6 +433,18 @@ int check_opts(const char* what, const rs_embed_opts* o) {
   return RS_OK;
 }
 
+// Whether `bytes` at `out` touch one of n rows of `width` bytes, `pitch` apart.
+bool touches_rows(uint64_t rows, int64_t n, uint64_t pitch, uint64_t width, uint64_t out, uint64_t bytes) {
+  if (n == 0 || width == 0 || bytes == 0 || out + bytes <= rows) return false;
+  // the first row that ends past `out`
+  uint64_t i = 0;
+  if (rows + width <= out) {
+    if (pitch == 0) return false;
+    i = (out - rows - width) / pitch + 1;
+  }
+  return i < (uint64_t)n && rows + i * pitch < out + bytes;
+}
+
 struct GradPlan {
   int cluster = 1, items = 1, tiles = 0;
   uint64_t keys = 0, toks = 0, partial = 0, long_rows = 0, bytes = 0;
@@ -548,18 +560,25 @@ int rs_embed_grad(const rs_embed_opts* opts, const void* ids_dev, const void* gr
     if (o.rows == 0 || o.hidden == 0) return RS_OK;
     const int b = dtype_bytes(o.dtype), gb = dtype_bytes(o.grad_dtype);
     if (!grad_dev || (uint64_t)grad_dev % gb) return tfail(RS_ERR_ARG, "rs_embed_grad: NULL or misaligned gradient");
-    DeviceGuard guard(device);
-    if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_embed_grad: cudaSetDevice");
-    const int sms = sm_count(device);
     cudaStream_t st = (cudaStream_t)stream;
     const uint64_t out_bytes = (uint64_t)o.rows * o.hidden * gb;
-    if (o.n_tokens == 0)
-      return o.accumulate ? RS_OK : tcuda(cudaMemsetAsync(grad_dev, 0, out_bytes, st), "rs_embed_grad: cudaMemsetAsync");
+    if (o.n_tokens == 0) {
+      if (o.accumulate) return RS_OK;
+      DeviceGuard guard(device);
+      if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_embed_grad: cudaSetDevice");
+      return tcuda(cudaMemsetAsync(grad_dev, 0, out_bytes, st), "rs_embed_grad: cudaMemsetAsync");
+    }
     if (!ids_dev || !grad_out_dev || (uint64_t)ids_dev % (o.wide_ids ? 8 : 4) || (uint64_t)grad_out_dev % b)
       return tfail(RS_ERR_ARG, "rs_embed_grad: NULL or misaligned ids or output gradient");
+    // the output is cleared and written while these rows are read
+    if (touches_rows((uint64_t)grad_out_dev, o.n_tokens, (uint64_t)o.grad_stride * b, (uint64_t)o.hidden * b, (uint64_t)grad_dev, out_bytes))
+      return tfail(RS_ERR_ARG, "rs_embed_grad: the gradient overlaps the output's gradient");
     const GradPlan p = plan_grad(o);
     if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 256)
       return tfail(RS_ERR_CAPACITY, "rs_embed_grad: workspace too small or not 256-byte aligned");
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_embed_grad: cudaSetDevice");
+    const int sms = sm_count(device);
     char* ws = (char*)workspace;
     SortArgs s{};
     s.ids = ids_dev;

@@ -75,12 +75,24 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, lo
     return _lookup(ids, weight, scale, lo, group)
 
 
+def _touches(g: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether the contiguous `out` shares memory with a row of g, [n, hidden] with contiguous rows."""
+    size = g.element_size()
+    pitch, width = g.stride(0) * size, g.shape[1] * size
+    lo, hi = out.data_ptr() - g.data_ptr(), out.data_ptr() - g.data_ptr() + out.numel() * out.element_size()
+    if not g.numel() or not out.numel() or (pitch == 0 and lo >= width):
+        return False
+    i = max(0, (lo - width) // pitch + 1) if lo >= width else 0  # the first row that ends past lo
+    return i < g.shape[0] and i * pitch < hi
+
+
 def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, rows: int, *, scale: float = 1.0, lo: int = 0,
                    dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """The gradient of embedding()'s weight, [rows, hidden]: row r is scale * the sum of grad_out over
     the tokens with id lo + r, summed in 32 bits in an order that the ids alone fix, and rounded
-    once to `dtype` (default: grad_out's, or out's). `out` (contiguous) receives it; with accumulate=True it is
-    added to what `out` holds. Rows without a token are 0 (left alone when accumulating).
+    once to `dtype` (default: grad_out's, or out's). `out` (contiguous, sharing no memory with
+    grad_out) receives it; with accumulate=True it is added to what `out` holds. Rows without a token
+    are 0 (left alone when accumulating).
 
     More than 65536 tokens are taken in parts of that many; for a 16-bit gradient the parts meet in a
     float32 one, so that it is rounded once all the same."""
@@ -91,6 +103,10 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, rows: int, *, scal
     if tuple(grad_out.shape[:-1]) != tuple(ids.shape):
         raise AssertionError(f"grad_out has shape {list(grad_out.shape)}, ids {list(ids.shape)}")
     g, flat = grad_out.reshape(-1, hidden), ids.reshape(-1)
+    if hidden > 1 and g.stride(1) != 1:
+        g = g.contiguous()
+    if out is not None and _touches(g, out):
+        raise L.ReshardError(L.RS_ERR_ARG, "embedding_grad: the gradient overlaps the output's gradient")
     out = L.extension().embed_grad(g[:0], flat[:0], rows, scale, lo, dtype, out, accumulate)
     wide = out if out.dtype == torch.float32 else torch.zeros(out.shape, dtype=torch.float32, device=out.device)
     for at in range(0, n, _MAX_SORTED):

@@ -289,3 +289,25 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
         V.embedding(ids, w), V.token_logprobs(z, t)  # tensors without a tangent
+
+
+# ---- memory used twice, and sizes of nothing ------------------------------------------------------
+@pytest.mark.parametrize("n", [100, 70000])
+def test_a_gradient_over_its_own_input_is_refused(n):
+    """The output is cleared and written while grad_out is read."""
+    for dtype in (F32, BF16):
+        buf = randn(n + 64, 16, dtype=dtype, seed=1)
+        ids = torch.randint(0, 64, (n,), generator=gen(1), device=DEV)
+        kept = buf.clone()
+        for g, out in ((buf[:n], buf[:64]), (buf[:n], buf[n - 64:n]), (buf[:n], buf[n - 1:n + 63]), (buf[:n, :8], buf.view(-1)[:512].view(64, 8)),
+                       (buf[:1].expand(n, 16), buf[:64])):
+            for acc in (False, True):
+                with pytest.raises(RuntimeError, match="overlaps"):
+                    V.embedding_grad(g, ids, 64, out=out, accumulate=acc)
+        assert torch.equal(buf, kept)
+        out = buf[n:]  # beside it
+        assert torch.equal(V.embedding_grad(buf[:n], ids, 64, out=out), V.embedding_grad(kept[:n], ids, 64, dtype=dtype))
+        one = torch.where(ids == 3, 0, -1)  # between two of its rows
+        wide = kept.clone()
+        got = V.embedding_grad(wide[:n, :8], one, 1, out=wide[5:6, 8:])
+        assert torch.equal(got, V.embedding_grad(kept[:n, :8].contiguous(), one, 1))

@@ -1,7 +1,10 @@
 """Refusals of the training-step operators that are made before any CUDA call."""
 import ctypes
 
+import torch
+
 from suika_b200 import _lib as L
+from suika_b200 import vocab as V
 
 FAKE = 1 << 20  # an address that no check dereferences
 
@@ -28,3 +31,34 @@ def test_record_entry_checks_its_index_base():
     for base in ((1 << 31) - 8, 1 << 31, (1 << 63) - 1):
         assert call(base) == L.RS_ERR_CAPACITY, base
     assert call((1 << 31) - 9) == L.RS_ERR_ARG and b"NULL" in lib.rs_last_error()
+
+
+def _rows_meet(rows, n, pitch, width, out, size):
+    return any(rows + i * pitch < out + size and out < rows + i * pitch + width for i in range(n)) and width > 0 and size > 0
+
+
+def test_embedding_gradient_entry_refuses_its_own_input():
+    """Every place of a small output about a few rows, with gaps, without, and on top of one another, against a search."""
+    lib = L.load()
+    for n, stride, hidden in ((1, 8, 8), (3, 8, 8), (3, 12, 8), (3, 0, 8), (4, 6, 8)):
+        for out_rows in (1, 2):
+            for at in range(-24, 60):
+                rows, out = FAKE, FAKE + 4 * at
+                o = L.RsEmbedOpts(n, out_rows, hidden, 0, hidden, stride, 1.0, L.RS_F32, L.RS_F32, 1, 0, 0)
+                rc = lib.rs_embed_grad(ctypes.byref(o), FAKE * 2, rows, out, None, 0, 0, None)
+                meet = _rows_meet(rows, n, 4 * stride, 4 * hidden, out, 4 * hidden * out_rows)
+                assert rc == (L.RS_ERR_ARG if meet else L.RS_ERR_CAPACITY), (n, stride, out_rows, at, lib.rs_last_error())  # no workspace was given
+                if meet:
+                    assert b"overlaps" in lib.rs_last_error()
+
+
+def test_embedding_gradient_of_long_batches_refuses_its_own_input():
+    whole = torch.zeros(200)
+    for n, stride, hidden in ((1, 8, 8), (3, 8, 8), (3, 12, 8), (3, 0, 8), (4, 6, 8), (5, 1, 1)):
+        g = whole[40:].as_strided((n, hidden), (stride, 1), 40)
+        for out_rows in (1, 2):
+            for at in range(0, 150):
+                out = whole[at:at + out_rows * hidden].view(out_rows, hidden)
+                meet = _rows_meet(40, n, stride, hidden, at, out_rows * hidden)
+                assert V._touches(g, out) == meet, (n, stride, hidden, out_rows, at)
+    assert not V._touches(whole[:0].view(0, 4), whole[:8].view(2, 4)) and not V._touches(whole[:8].view(2, 4), whole[:0].view(0, 4))
