@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/util/accumulate.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -115,7 +116,7 @@ std::string shape_of(at::IntArrayRef s) {
 }
 // [..., cols] as rows of `cols` contiguous elements; copies only what no stride describes.
 at::Tensor as_rows(const at::Tensor& t, int64_t cols) {
-  at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, cols});
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), cols});
   return r.stride(1) == 1 || cols < 2 ? r : r.contiguous();
 }
 

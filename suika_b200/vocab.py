@@ -102,7 +102,7 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, rows: int, *, scal
     n, hidden = ids.numel(), grad_out.shape[-1]
     if tuple(grad_out.shape[:-1]) != tuple(ids.shape):
         raise AssertionError(f"grad_out has shape {list(grad_out.shape)}, ids {list(ids.shape)}")
-    g, flat = grad_out.reshape(-1, hidden), ids.reshape(-1)
+    g, flat = grad_out.reshape(n, hidden), ids.reshape(-1)
     if hidden > 1 and g.stride(1) != 1:
         g = g.contiguous()
     if out is not None and _touches(g, out):

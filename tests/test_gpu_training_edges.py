@@ -311,3 +311,10 @@ def test_a_gradient_over_its_own_input_is_refused(n):
         wide = kept.clone()
         got = V.embedding_grad(wide[:n, :8], one, 1, out=wide[5:6, 8:])
         assert torch.equal(got, V.embedding_grad(kept[:n, :8].contiguous(), one, 1))
+
+
+def test_gradient_of_no_columns():
+    for n in (3, 70000):
+        ids = torch.zeros(2, n, dtype=torch.int64, device=DEV)
+        assert V.embedding_grad(torch.zeros(2, n, 0, device=DEV), ids, 5).shape == (5, 0)
+        assert V.embedding(ids, torch.zeros(5, 0, device=DEV)).shape == (2, n, 0)
