@@ -45,6 +45,14 @@ PyObject* entry(F&& body) {
     return body();
   } catch (const Raise& r) {
     if (r.type) PyErr_SetString(r.type, r.msg.c_str());
+  } catch (const c10::OutOfMemoryError& e) {  // as torch's own operators raise them: the class, and no C++ stack
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    if (type) PyErr_SetString(type, e.what_without_backtrace());
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
+  } catch (const c10::Error& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   } catch (...) {

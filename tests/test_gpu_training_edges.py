@@ -318,3 +318,13 @@ def test_gradient_of_no_columns():
         ids = torch.zeros(2, n, dtype=torch.int64, device=DEV)
         assert V.embedding_grad(torch.zeros(2, n, 0, device=DEV), ids, 5).shape == (5, 0)
         assert V.embedding(ids, torch.zeros(5, 0, device=DEV)).shape == (2, n, 0)
+
+
+# ---- errors of the allocator --------------------------------------------------------------------
+def test_out_of_memory_is_torchs_own_error():
+    """A call that finds no memory raises what torch's operators raise, without the library's stack."""
+    ids, w = torch.zeros(1 << 18, dtype=torch.int64, device=DEV), torch.zeros(1, 1 << 22, dtype=BF16, device=DEV)  # 2 TB
+    with pytest.raises(torch.OutOfMemoryError) as e:
+        V.embedding(ids, w)
+    assert "c10::" not in str(e.value)
+    assert torch.equal(V.embedding(ids[:2], w), w.expand(2, -1))
