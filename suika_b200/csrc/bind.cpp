@@ -28,15 +28,30 @@ struct Raise {
 [[noreturn]] void assertion_error(const std::string& m) { throw Raise{PyExc_AssertionError, m}; }
 [[noreturn]] void already_set() { throw Raise{nullptr, ""}; }
 
-// suika_b200._lib.check: the exception that belongs to a status.
+// A status on its way to suika_b200._lib.check, which raises the exception that belongs to it.
+struct Status {
+  int rc;
+};
 void check(int rc) {
-  if (rc == RS_OK) return;
+  if (rc != RS_OK) throw Status{rc};
+}
+void raise_status(int rc) {
   PyObject* lib = PyImport_ImportModule("suika_b200._lib");
   PyObject* r = lib ? PyObject_CallMethod(lib, "check", "i", rc) : nullptr;
   Py_XDECREF(r);
   Py_XDECREF(lib);
   if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, rs_last_error());
-  already_set();
+}
+
+// Allocation and launches run in `body` without the interpreter's lock: a full launch queue or a cudaMalloc
+// waits in the driver, and other Python threads go on. Nothing of Python is touched in there.
+template <class F>
+auto unlocked(F&& body) {
+  struct Unlock {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlock() { PyEval_RestoreThread(state); }
+  } unlock;
+  return body();
 }
 
 template <class F>
@@ -45,6 +60,8 @@ PyObject* entry(F&& body) {
     return body();
   } catch (const Raise& r) {
     if (r.type) PyErr_SetString(r.type, r.msg.c_str());
+  } catch (const Status& s) {
+    raise_status(s.rc);
   } catch (const c10::OutOfMemoryError& e) {  // as torch's own operators raise them: the class, and no C++ stack
     PyObject* torch = PyImport_ImportModule("torch");
     PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
@@ -138,21 +155,24 @@ PyObject* embed_lookup(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t rows = weight.size(0), hidden = weight.size(1);
     const uint32_t code = dtype_code(weight, "weight");
     if (weight.stride(1) != 1 && hidden > 1) value_error("weight must have contiguous rows");
-    const at::Tensor ids = index_tensor(tensor(a[0], "ids"), weight, "ids");
-    std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
-    shape.push_back(hidden);
-    at::Tensor out = at::empty(shape, weight.options());
+    const at::Tensor& given_ids = tensor(a[0], "ids");
     rs_embed_opts o{};
-    o.n_tokens = ids.numel();
     o.rows = rows;
     o.hidden = hidden;
     o.lo = integer(a[3]);
     o.weight_stride = weight.stride(0);
     o.scale = (float)number(a[2]);
     o.dtype = o.grad_dtype = code;
-    o.wide_ids = ids.scalar_type() == at::kLong;
-    check(rs_embed_lookup(&o, ids.data_ptr(), weight.data_ptr(), out.data_ptr(), weight.get_device(), stream_of(weight)));
-    return THPVariable_Wrap(std::move(out));
+    return THPVariable_Wrap(unlocked([&] {
+      const at::Tensor ids = index_tensor(given_ids, weight, "ids");
+      std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
+      shape.push_back(hidden);
+      at::Tensor out = at::empty(shape, weight.options());
+      o.n_tokens = ids.numel();
+      o.wide_ids = ids.scalar_type() == at::kLong;
+      check(rs_embed_lookup(&o, ids.data_ptr(), weight.data_ptr(), out.data_ptr(), weight.get_device(), stream_of(weight)));
+      return out;
+    }));
   });
 }
 
@@ -166,41 +186,45 @@ PyObject* embed_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t hidden = grad_out.size(-1), rows = integer(a[2]);
     rs_embed_opts o{};
     o.dtype = dtype_code(grad_out, "grad_out");
-    const at::Tensor ids = index_tensor(tensor(a[1], "ids"), grad_out, "ids");
-    if (grad_out.sizes().slice(0, grad_out.dim() - 1) != ids.sizes())
-      assertion_error("grad_out has shape " + shape_of(grad_out.sizes()) + ", ids " + shape_of(ids.sizes()));
+    const at::Tensor& given_ids = tensor(a[1], "ids");
     o.accumulate = truth(a[7]);
+    o.lo = integer(a[4]);
+    o.scale = (float)number(a[3]);
     const bool has_dtype = a[5] != Py_None;
     if (has_dtype && !THPDtype_Check(a[5])) throw Raise{PyExc_TypeError, "dtype must be a torch.dtype"};
     const at::ScalarType dtype = has_dtype ? reinterpret_cast<THPDtype*>(a[5])->scalar_type : grad_out.scalar_type();
     at::Tensor out;
-    if (a[6] == Py_None) {
-      if (o.accumulate) value_error("accumulate=True adds to `out`: give one");
-      if (rows < 0) value_error("a negative number of rows");
-      out = at::empty({rows, hidden}, grad_out.options().dtype(dtype));
-    } else {
-      out = tensor(a[6], "out");
-      if (out.device() != grad_out.device() || !out.is_contiguous()) value_error("out must be contiguous and on grad_out's device");
-      if (out.dim() != 2 || out.size(0) != rows || out.size(1) != hidden)
-        assertion_error("out has shape " + shape_of(out.sizes()) + ", expected " + shape_of({rows, hidden}));
-      if (has_dtype && out.scalar_type() != dtype) value_error("out of " + type_name(out) + ", but a gradient of another type is asked for");
-    }
-    o.grad_dtype = dtype_code(out, "the gradient");
-    const at::Tensor g = as_rows(grad_out, hidden);
-    o.n_tokens = ids.numel();
-    o.rows = rows;
-    o.hidden = hidden;
-    o.lo = integer(a[4]);
-    o.grad_stride = g.stride(0);
-    o.scale = (float)number(a[3]);
-    o.wide_ids = ids.scalar_type() == at::kLong;
-    const int device = grad_out.get_device();
-    uint64_t bytes = 0;
-    check(rs_embed_grad_workspace_bytes(&o, device, &bytes));
-    const at::Tensor workspace = at::empty({(int64_t)bytes}, grad_out.options().dtype(at::kByte));
-    check(rs_embed_grad(&o, ids.data_ptr(), g.data_ptr(), out.data_ptr(), workspace.data_ptr(), bytes, device, stream_of(grad_out)));
-    if (a[6] != Py_None) written(out);
-    return THPVariable_Wrap(std::move(out));
+    if (a[6] != Py_None) out = tensor(a[6], "out");
+    return THPVariable_Wrap(unlocked([&] {
+      const at::Tensor ids = index_tensor(given_ids, grad_out, "ids");
+      if (grad_out.sizes().slice(0, grad_out.dim() - 1) != ids.sizes())
+        assertion_error("grad_out has shape " + shape_of(grad_out.sizes()) + ", ids " + shape_of(ids.sizes()));
+      const bool given = out.defined();
+      if (!given) {
+        if (o.accumulate) value_error("accumulate=True adds to `out`: give one");
+        if (rows < 0) value_error("a negative number of rows");
+        out = at::empty({rows, hidden}, grad_out.options().dtype(dtype));
+      } else {
+        if (out.device() != grad_out.device() || !out.is_contiguous()) value_error("out must be contiguous and on grad_out's device");
+        if (out.dim() != 2 || out.size(0) != rows || out.size(1) != hidden)
+          assertion_error("out has shape " + shape_of(out.sizes()) + ", expected " + shape_of({rows, hidden}));
+        if (has_dtype && out.scalar_type() != dtype) value_error("out of " + type_name(out) + ", but a gradient of another type is asked for");
+      }
+      o.grad_dtype = dtype_code(out, "the gradient");
+      const at::Tensor g = as_rows(grad_out, hidden);
+      o.n_tokens = ids.numel();
+      o.rows = rows;
+      o.hidden = hidden;
+      o.grad_stride = g.stride(0);
+      o.wide_ids = ids.scalar_type() == at::kLong;
+      const int device = grad_out.get_device();
+      uint64_t bytes = 0;
+      check(rs_embed_grad_workspace_bytes(&o, device, &bytes));
+      const at::Tensor workspace = at::empty({(int64_t)bytes}, grad_out.options().dtype(at::kByte));
+      check(rs_embed_grad(&o, ids.data_ptr(), g.data_ptr(), out.data_ptr(), workspace.data_ptr(), bytes, device, stream_of(grad_out)));
+      if (given) written(out);
+      return out;
+    }));
   });
 }
 
@@ -238,20 +262,23 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return entry([&]() -> PyObject* {
     count_args("token_logprobs", n, 4);
     const int64_t top = top_of(a[2]);
-    const at::Tensor& logits = tensor(a[0], "logits");
-    const Logits l(logits, tensor(a[1], "targets"), top, integer(a[3]), false);
-    const auto f32 = logits.options().dtype(at::kFloat);
+    const at::Tensor &logits = tensor(a[0], "logits"), &targets = tensor(a[1], "targets");
+    const int64_t lo = integer(a[3]);
     at::Tensor out[5];
-    for (int i = 0; i < 3; ++i) out[i] = at::empty(l.targets.sizes(), f32);
-    if (top) {
-      std::vector<int64_t> shape(l.targets.sizes().begin(), l.targets.sizes().end());
-      shape.push_back(top);
-      out[3] = at::empty(shape, f32);
-      out[4] = at::empty(shape, logits.options().dtype(at::kLong));
-    }
-    check(rs_token_logprobs(&l.o, l.z.data_ptr(), l.targets.data_ptr(), out[0].data_ptr<float>(), out[1].data_ptr<float>(), out[2].data_ptr<float>(),
-                            top ? out[3].data_ptr<float>() : nullptr, top ? out[4].data_ptr<int64_t>() : nullptr, logits.get_device(),
-                            stream_of(logits)));
+    unlocked([&] {
+      const Logits l(logits, targets, top, lo, false);
+      const auto f32 = logits.options().dtype(at::kFloat);
+      for (int i = 0; i < 3; ++i) out[i] = at::empty(l.targets.sizes(), f32);
+      if (top) {
+        std::vector<int64_t> shape(l.targets.sizes().begin(), l.targets.sizes().end());
+        shape.push_back(top);
+        out[3] = at::empty(shape, f32);
+        out[4] = at::empty(shape, logits.options().dtype(at::kLong));
+      }
+      check(rs_token_logprobs(&l.o, l.z.data_ptr(), l.targets.data_ptr(), out[0].data_ptr<float>(), out[1].data_ptr<float>(),
+                              out[2].data_ptr<float>(), top ? out[3].data_ptr<float>() : nullptr, top ? out[4].data_ptr<int64_t>() : nullptr,
+                              logits.get_device(), stream_of(logits)));
+    });
     PyObject* r = PyTuple_New(5);
     if (!r) already_set();
     for (int i = 0; i < 5; ++i) {
@@ -267,11 +294,14 @@ PyObject* token_record(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return entry([&]() -> PyObject* {
     count_args("token_record", n, 5);
     const int64_t top = top_of(a[2]);
-    const at::Tensor& logits = tensor(a[0], "logits");
-    const Logits l(logits, tensor(a[1], "targets"), top, integer(a[3]), true);
-    at::Tensor out = at::empty({l.o.n_rows, 4 + 2 * top}, logits.options().dtype(at::kFloat));
-    check(rs_token_record_at(&l.o, integer(a[4]), l.z.data_ptr(), l.targets.data_ptr(), out.data_ptr<float>(), logits.get_device(), stream_of(logits)));
-    return THPVariable_Wrap(std::move(out));
+    const at::Tensor &logits = tensor(a[0], "logits"), &targets = tensor(a[1], "targets");
+    const int64_t lo = integer(a[3]), index_base = integer(a[4]);
+    return THPVariable_Wrap(unlocked([&] {
+      const Logits l(logits, targets, top, lo, true);
+      at::Tensor out = at::empty({l.o.n_rows, 4 + 2 * top}, logits.options().dtype(at::kFloat));
+      check(rs_token_record_at(&l.o, index_base, l.z.data_ptr(), l.targets.data_ptr(), out.data_ptr<float>(), logits.get_device(), stream_of(logits)));
+      return out;
+    }));
   });
 }
 
@@ -280,34 +310,44 @@ PyObject* token_record(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* token_logprobs_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return entry([&]() -> PyObject* {
     count_args("token_logprobs_grad", n, 12);
-    const at::Tensor& logits = tensor(a[0], "logits");
-    const Logits l(logits, tensor(a[1], "targets"), 0, integer(a[7]), truth(a[8]));
+    const at::Tensor &logits = tensor(a[0], "logits"), &targets = tensor(a[1], "targets");
+    const int64_t lo = integer(a[7]);
+    const bool sharded = truth(a[8]), ranged = a[10] != Py_None;
+    const int64_t first = ranged ? integer(a[10]) : 0, end = ranged ? integer(a[11]) : 0;
+    need_cuda(logits, "logits");
     if (a[5] != Py_None && a[3] == Py_None) value_error("a gradient of the entropy needs the entropy");
     if (a[2] == Py_None || a[4] == Py_None) value_error("lse and grad_logprob are needed");
     static const char* names[5] = {"lse", "entropy", "grad_logprob", "grad_entropy", "grad_lse"};
-    at::Tensor rows[5];
-    const float* p[5] = {};
-    for (int i = 0; i < 5; ++i) {
-      if (a[2 + i] == Py_None) continue;
-      const at::Tensor& t = tensor(a[2 + i], names[i]);
-      if (t.sizes() != l.targets.sizes() || t.scalar_type() != at::kFloat || t.device() != logits.device())
-        value_error(std::string(names[i]) + " must be float32, of targets' shape and on their device");
-      rows[i] = t.contiguous();
-      p[i] = rows[i].data_ptr<float>();
-    }
-    at::Tensor out = a[9] == Py_None ? at::empty(logits.sizes(), logits.options()) : tensor(a[9], "out");
-    if (a[9] != Py_None && (out.sizes() != logits.sizes() || out.scalar_type() != logits.scalar_type() || out.device() != logits.device()))
-      value_error("out must have the logits' shape, type and device");
-    const at::Tensor o = out.dim() == 2 ? out : out.view({-1, l.o.cols});
-    if (o.stride(1) != 1 && l.o.cols > 1) value_error("out must have contiguous rows");
-    if (a[10] == Py_None)
-      check(rs_token_logprobs_grad(&l.o, l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4], o.data_ptr(), o.stride(0),
-                                   logits.get_device(), stream_of(logits)));
-    else
-      check(rs_token_logprobs_shard_grad(&l.o, integer(a[10]), integer(a[11]), l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4],
-                                         o.data_ptr(), o.stride(0), logits.get_device(), stream_of(logits)));
-    if (a[9] != Py_None) written(out);
-    return THPVariable_Wrap(std::move(out));
+    at::Tensor rows[5], out;
+    for (int i = 0; i < 5; ++i)
+      if (a[2 + i] != Py_None) rows[i] = tensor(a[2 + i], names[i]);
+    if (a[9] != Py_None) out = tensor(a[9], "out");
+    return THPVariable_Wrap(unlocked([&] {
+      const Logits l(logits, targets, 0, lo, sharded);
+      const float* p[5] = {};
+      for (int i = 0; i < 5; ++i) {
+        at::Tensor& t = rows[i];
+        if (!t.defined()) continue;
+        if (t.sizes() != l.targets.sizes() || t.scalar_type() != at::kFloat || t.device() != logits.device())
+          value_error(std::string(names[i]) + " must be float32, of targets' shape and on their device");
+        t = t.contiguous();
+        p[i] = t.data_ptr<float>();
+      }
+      const bool given = out.defined();
+      if (!given) out = at::empty(logits.sizes(), logits.options());
+      if (out.sizes() != logits.sizes() || out.scalar_type() != logits.scalar_type() || out.device() != logits.device())
+        value_error("out must have the logits' shape, type and device");
+      const at::Tensor o = out.dim() == 2 ? out : out.view({-1, l.o.cols});
+      if (o.stride(1) != 1 && l.o.cols > 1) value_error("out must have contiguous rows");
+      if (!ranged)
+        check(rs_token_logprobs_grad(&l.o, l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4], o.data_ptr(), o.stride(0),
+                                     logits.get_device(), stream_of(logits)));
+      else
+        check(rs_token_logprobs_shard_grad(&l.o, first, end, l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4], o.data_ptr(),
+                                           o.stride(0), logits.get_device(), stream_of(logits)));
+      if (given) written(out);
+      return out;
+    }));
   });
 }
 
@@ -357,10 +397,12 @@ PyObject* grad_sumsq(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[1] != Py_None && PyList_Check(a[0]) && PyList_GET_SIZE(a[0]) == 0) {
       const at::Tensor& like = tensor(a[1], "gradients");
       need_cuda(like, "gradients");
-      return THPVariable_Wrap(sumsq_of({}, like));
+      return THPVariable_Wrap(unlocked([&] { return sumsq_of({}, like); }));
     }
     const auto ts = tensors_of(a[0], "gradients");
-    return THPVariable_Wrap(sumsq_of(spans_of(ts), *ts[0]));
+    const auto s = spans_of(ts);
+    const at::Tensor first = *ts[0];  // the list may change meanwhile
+    return THPVariable_Wrap(unlocked([&] { return sumsq_of(s, first); }));
   });
 }
 
@@ -370,14 +412,18 @@ PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
     count_args("grad_clip", n, 3);
     const auto ts = tensors_of(a[0], "gradients");
     const auto s = spans_of(ts);
-    const at::Tensor& first = *ts[0];
+    const at::Tensor first = *ts[0];
     const float max_norm = (float)number(a[1]);
-    const at::Tensor sumsq = a[2] == Py_None ? sumsq_of(s, first) : tensor(a[2], "sumsq");
-    at::Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
-    check(rs_grad_clip(s.data(), (int64_t)s.size(), given_sumsq(sumsq, first), max_norm, norm.data_ptr<float>(), first.get_device(),
-                       stream_of(first)));
-    for (const at::Tensor* t : ts) written(*t);
-    return THPVariable_Wrap(std::move(norm));
+    at::Tensor sumsq;
+    if (a[2] != Py_None) sumsq = tensor(a[2], "sumsq");
+    for (const at::Tensor* t : ts) written(*t);  // here, since the list may change while the lock is let go
+    return THPVariable_Wrap(unlocked([&] {
+      if (!sumsq.defined()) sumsq = sumsq_of(s, first);
+      at::Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
+      check(rs_grad_clip(s.data(), (int64_t)s.size(), given_sumsq(sumsq, first), max_norm, norm.data_ptr<float>(), first.get_device(),
+                         stream_of(first)));
+      return norm;
+    }));
   });
 }
 
@@ -390,7 +436,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (int i = 0; i < 7; ++i)
       if (!PyList_Check(a[i]) || PyList_GET_SIZE(a[i]) != PyList_GET_SIZE(a[0])) throw Raise{PyExc_TypeError, "lists of one length are taken"};
     const auto ts = tensors_of(a[6], "gradients");
-    const at::Tensor& first = *ts[0];
+    const at::Tensor first = *ts[0];
     const double decay = number(a[11]);
     std::vector<rs_adamw_tensor> t;
     t.reserve(ts.size());
@@ -434,18 +480,20 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         sumsq = tensor(a[13], "sumsq");
         given_sumsq(sumsq, first);
       }
-      norm = at::empty({}, first.options().dtype(at::kFloat));
     }
-    uint64_t bytes = 0;
-    check(rs_adamw_workspace_bytes((int64_t)t.size(), &bytes));
-    const at::Tensor workspace = at::empty({(int64_t)bytes}, first.options().dtype(at::kByte));
-    check(rs_adamw_step(t.data(), (int64_t)t.size(), &o, sumsq.defined() ? sumsq.data_ptr<double>() : nullptr, clip ? norm.data_ptr<float>() : nullptr,
-                        workspace.data_ptr(), bytes, first.get_device(), stream_of(first)));
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[6]); ++i) {
       if (PyList_GET_ITEM(a[6], i) == Py_None) continue;
       for (int list = 0; list < 5; ++list)
         if (PyList_GET_ITEM(a[list], i) != Py_None) written(tensor(PyList_GET_ITEM(a[list], i), "a sub-field"));
     }
+    unlocked([&] {
+      if (clip) norm = at::empty({}, first.options().dtype(at::kFloat));
+      uint64_t bytes = 0;
+      check(rs_adamw_workspace_bytes((int64_t)t.size(), &bytes));
+      const at::Tensor workspace = at::empty({(int64_t)bytes}, first.options().dtype(at::kByte));
+      check(rs_adamw_step(t.data(), (int64_t)t.size(), &o, sumsq.defined() ? sumsq.data_ptr<double>() : nullptr,
+                          clip ? norm.data_ptr<float>() : nullptr, workspace.data_ptr(), bytes, first.get_device(), stream_of(first)));
+    });
     return clip ? THPVariable_Wrap(std::move(norm)) : Py_NewRef(Py_None);
   });
 }

@@ -5,6 +5,8 @@ import json
 import math
 import os
 import tempfile
+import threading
+import time
 import traceback
 
 import pytest
@@ -328,3 +330,35 @@ def test_out_of_memory_is_torchs_own_error():
         V.embedding(ids, w)
     assert "c10::" not in str(e.value)
     assert torch.equal(V.embedding(ids[:2], w), w.expand(2, -1))
+
+
+# ---- other threads ------------------------------------------------------------------------------
+def test_other_threads_run_while_a_call_waits_for_the_launch_queue():
+    """A call that finds the launch queue full waits in the driver; Python goes on meanwhile."""
+    w, ids = randn(50, 64, seed=1), torch.arange(8, device=DEV)
+    V.embedding(ids, w)
+    torch.cuda.synchronize()
+    gaps, stop = [0.0], threading.Event()
+
+    def count():
+        last = time.perf_counter()
+        while not stop.is_set():
+            now = time.perf_counter()
+            gaps[0] = max(gaps[0], now - last)
+            last = now
+            time.sleep(0.001)
+    other = threading.Thread(target=count)
+    other.start()
+    torch.cuda._sleep(1_500_000_000)  # about 0.8 s of a kernel that does nothing
+    longest = 0.0
+    for _ in range(6000):
+        t0 = time.perf_counter()
+        V.embedding(ids, w)
+        longest = max(longest, time.perf_counter() - t0)
+    stop.set()
+    other.join()
+    torch.cuda.synchronize()
+    print(f"longest call {longest:.3f} s, the other thread's longest wait {gaps[0]:.3f} s")
+    if longest < 0.2:
+        pytest.skip("the launch queue did not fill")
+    assert gaps[0] < longest / 2
