@@ -122,11 +122,11 @@ uint32_t dtype_code(const at::Tensor& t, const char* what) {
 void need_cuda(const at::Tensor& t, const char* what) {
   if (!t.is_cuda()) value_error(std::string(what) + " must be a CUDA tensor");
 }
-at::Tensor index_tensor(const at::Tensor& t, const at::Tensor& with, const char* what) {
+c10::MaybeOwned<at::Tensor> index_tensor(const at::Tensor& t, const at::Tensor& with, const char* what) {
   if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)
     value_error(std::string(what) + " of " + type_name(t) + ": int64 and int32 are taken");
   if (t.device() != with.device()) value_error(std::string(what) + " must be on the device of the other tensors");
-  return t.contiguous();
+  return t.expect_contiguous();
 }
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 // A tensor that a kernel wrote in place counts as written for autograd, as after torch's own in-place operators: a
@@ -164,7 +164,8 @@ PyObject* embed_lookup(PyObject*, PyObject* const* a, Py_ssize_t n) {
     o.scale = (float)number(a[2]);
     o.dtype = o.grad_dtype = code;
     return THPVariable_Wrap(unlocked([&] {
-      const at::Tensor ids = index_tensor(given_ids, weight, "ids");
+      const auto held = index_tensor(given_ids, weight, "ids");
+      const at::Tensor& ids = *held;
       std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
       shape.push_back(hidden);
       at::Tensor out = at::empty(shape, weight.options());
@@ -196,7 +197,8 @@ PyObject* embed_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor out;
     if (a[6] != Py_None) out = tensor(a[6], "out");
     return THPVariable_Wrap(unlocked([&] {
-      const at::Tensor ids = index_tensor(given_ids, grad_out, "ids");
+      const auto held = index_tensor(given_ids, grad_out, "ids");
+      const at::Tensor& ids = *held;
       if (grad_out.sizes().slice(0, grad_out.dim() - 1) != ids.sizes())
         assertion_error("grad_out has shape " + shape_of(grad_out.sizes()) + ", ids " + shape_of(ids.sizes()));
       const bool given = out.defined();
@@ -230,14 +232,15 @@ PyObject* embed_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---- token log probabilities ------------------------------------------------------------------
 struct Logits {
-  at::Tensor z, targets;
+  at::Tensor z;
+  c10::MaybeOwned<at::Tensor> targets;
   rs_logprob_opts o{};
   Logits(const at::Tensor& logits, const at::Tensor& t, int64_t top, int64_t lo, bool sharded) {
     need_cuda(logits, "logits");
     o.dtype = dtype_code(logits, "logits");
     targets = index_tensor(t, logits, "targets");
-    if (logits.dim() < 1 || logits.sizes().slice(0, logits.dim() - 1) != targets.sizes())
-      assertion_error("logits have shape " + shape_of(logits.sizes()) + ", targets " + shape_of(targets.sizes()));
+    if (logits.dim() < 1 || logits.sizes().slice(0, logits.dim() - 1) != t.sizes())
+      assertion_error("logits have shape " + shape_of(logits.sizes()) + ", targets " + shape_of(t.sizes()));
     const int64_t cols = logits.size(-1);
     if (cols == 0) value_error("logits of no columns");
     z = as_rows(logits, cols);
@@ -245,7 +248,7 @@ struct Logits {
     o.cols = cols;
     o.stride = z.stride(0);
     o.lo = lo;
-    o.wide_targets = targets.scalar_type() == at::kLong;
+    o.wide_targets = t.scalar_type() == at::kLong;
     o.top = (int32_t)top;
     o.sharded = sharded;
   }
@@ -268,14 +271,14 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     unlocked([&] {
       const Logits l(logits, targets, top, lo, false);
       const auto f32 = logits.options().dtype(at::kFloat);
-      for (int i = 0; i < 3; ++i) out[i] = at::empty(l.targets.sizes(), f32);
+      for (int i = 0; i < 3; ++i) out[i] = at::empty(targets.sizes(), f32);
       if (top) {
-        std::vector<int64_t> shape(l.targets.sizes().begin(), l.targets.sizes().end());
+        std::vector<int64_t> shape(targets.sizes().begin(), targets.sizes().end());
         shape.push_back(top);
         out[3] = at::empty(shape, f32);
         out[4] = at::empty(shape, logits.options().dtype(at::kLong));
       }
-      check(rs_token_logprobs(&l.o, l.z.data_ptr(), l.targets.data_ptr(), out[0].data_ptr<float>(), out[1].data_ptr<float>(),
+      check(rs_token_logprobs(&l.o, l.z.data_ptr(), l.targets->data_ptr(), out[0].data_ptr<float>(), out[1].data_ptr<float>(),
                               out[2].data_ptr<float>(), top ? out[3].data_ptr<float>() : nullptr, top ? out[4].data_ptr<int64_t>() : nullptr,
                               logits.get_device(), stream_of(logits)));
     });
@@ -299,7 +302,7 @@ PyObject* token_record(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return THPVariable_Wrap(unlocked([&] {
       const Logits l(logits, targets, top, lo, true);
       at::Tensor out = at::empty({l.o.n_rows, 4 + 2 * top}, logits.options().dtype(at::kFloat));
-      check(rs_token_record_at(&l.o, index_base, l.z.data_ptr(), l.targets.data_ptr(), out.data_ptr<float>(), logits.get_device(), stream_of(logits)));
+      check(rs_token_record_at(&l.o, index_base, l.z.data_ptr(), l.targets->data_ptr(), out.data_ptr<float>(), logits.get_device(), stream_of(logits)));
       return out;
     }));
   });
@@ -318,34 +321,36 @@ PyObject* token_logprobs_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[5] != Py_None && a[3] == Py_None) value_error("a gradient of the entropy needs the entropy");
     if (a[2] == Py_None || a[4] == Py_None) value_error("lse and grad_logprob are needed");
     static const char* names[5] = {"lse", "entropy", "grad_logprob", "grad_entropy", "grad_lse"};
-    at::Tensor rows[5], out;
+    const at::Tensor* given[5] = {};
     for (int i = 0; i < 5; ++i)
-      if (a[2 + i] != Py_None) rows[i] = tensor(a[2 + i], names[i]);
-    if (a[9] != Py_None) out = tensor(a[9], "out");
+      if (a[2 + i] != Py_None) given[i] = &tensor(a[2 + i], names[i]);
+    const bool has_out = a[9] != Py_None;
+    at::Tensor out;
+    if (has_out) out = tensor(a[9], "out");
     return THPVariable_Wrap(unlocked([&] {
       const Logits l(logits, targets, 0, lo, sharded);
+      c10::MaybeOwned<at::Tensor> rows[5];
       const float* p[5] = {};
       for (int i = 0; i < 5; ++i) {
-        at::Tensor& t = rows[i];
-        if (!t.defined()) continue;
-        if (t.sizes() != l.targets.sizes() || t.scalar_type() != at::kFloat || t.device() != logits.device())
+        if (!given[i]) continue;
+        const at::Tensor& t = *given[i];
+        if (t.sizes() != targets.sizes() || t.scalar_type() != at::kFloat || t.device() != logits.device())
           value_error(std::string(names[i]) + " must be float32, of targets' shape and on their device");
-        t = t.contiguous();
-        p[i] = t.data_ptr<float>();
+        rows[i] = t.expect_contiguous();
+        p[i] = rows[i]->data_ptr<float>();
       }
-      const bool given = out.defined();
-      if (!given) out = at::empty(logits.sizes(), logits.options());
+      if (!has_out) out = at::empty(logits.sizes(), logits.options());
       if (out.sizes() != logits.sizes() || out.scalar_type() != logits.scalar_type() || out.device() != logits.device())
         value_error("out must have the logits' shape, type and device");
       const at::Tensor o = out.dim() == 2 ? out : out.view({-1, l.o.cols});
       if (o.stride(1) != 1 && l.o.cols > 1) value_error("out must have contiguous rows");
       if (!ranged)
-        check(rs_token_logprobs_grad(&l.o, l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4], o.data_ptr(), o.stride(0),
+        check(rs_token_logprobs_grad(&l.o, l.z.data_ptr(), l.targets->data_ptr(), p[0], p[1], p[2], p[3], p[4], o.data_ptr(), o.stride(0),
                                      logits.get_device(), stream_of(logits)));
       else
-        check(rs_token_logprobs_shard_grad(&l.o, first, end, l.z.data_ptr(), l.targets.data_ptr(), p[0], p[1], p[2], p[3], p[4], o.data_ptr(),
+        check(rs_token_logprobs_shard_grad(&l.o, first, end, l.z.data_ptr(), l.targets->data_ptr(), p[0], p[1], p[2], p[3], p[4], o.data_ptr(),
                                            o.stride(0), logits.get_device(), stream_of(logits)));
-      if (given) written(out);
+      if (has_out) written(out);
       return out;
     }));
   });
@@ -439,27 +444,29 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor first = *ts[0];
     const double decay = number(a[11]);
     std::vector<rs_adamw_tensor> t;
+    std::vector<const at::Tensor*> updated;
     t.reserve(ts.size());
+    updated.reserve(5 * ts.size());
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[6]); ++i) {
       if (PyList_GET_ITEM(a[6], i) == Py_None) continue;
       const at::Tensor& g = *ts[t.size()];
-      const std::string who = "entry " + std::to_string(i) + " of the state: ";
+      auto who = [i] { return "entry " + std::to_string(i) + " of the state: "; };
       auto field = [&](int list, const char* what) -> const at::Tensor& {
         const at::Tensor& x = tensor(PyList_GET_ITEM(a[list], i), what);
         if (x.device() != g.device()) value_error("gradients must be on the state's device");
-        if (!x.is_contiguous()) value_error(who + what + " must be contiguous");
-        if (list < 4 && x.sizes() != g.sizes()) assertion_error(who + what + " and gradient differ in shape");
+        if (!x.is_contiguous()) value_error(who() + what + " must be contiguous");
+        if (list < 4 && x.sizes() != g.sizes()) assertion_error(who() + what + " and gradient differ in shape");
         return x;
       };
       const at::Tensor &p = field(0, "param"), &m = field(2, "exp_avg"), &v = field(3, "exp_avg_sq"), &step = field(4, "step");
-      const bool has_master = PyList_GET_ITEM(a[1], i) != Py_None;
-      if (m.scalar_type() != v.scalar_type()) value_error(who + "moments of two types");
-      if (step.scalar_type() != at::kFloat || step.numel() != 1) value_error(who + "the step must be one float32");
-      if (has_master && field(1, "master").scalar_type() != at::kFloat) value_error(who + "the master must be float32");
+      const at::Tensor* master = PyList_GET_ITEM(a[1], i) != Py_None ? &field(1, "master") : nullptr;
+      if (m.scalar_type() != v.scalar_type()) value_error(who() + "moments of two types");
+      if (step.scalar_type() != at::kFloat || step.numel() != 1) value_error(who() + "the step must be one float32");
+      if (master && master->scalar_type() != at::kFloat) value_error(who() + "the master must be float32");
       rs_adamw_tensor e{};
       e.grad_dev = (uint64_t)g.data_ptr();
       e.param_dev = (uint64_t)p.data_ptr();
-      e.master_dev = has_master ? (uint64_t)field(1, "master").data_ptr() : 0;
+      e.master_dev = master ? (uint64_t)master->data_ptr() : 0;
       e.exp_avg_dev = (uint64_t)m.data_ptr();
       e.exp_avg_sq_dev = (uint64_t)v.data_ptr();
       e.step_dev = (uint64_t)step.data_ptr();
@@ -469,6 +476,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       e.param_dtype = dtype_code(p, "param");
       e.moment_dtype = dtype_code(m, "exp_avg");
       t.push_back(e);
+      updated.insert(updated.end(), {&p, &m, &v, &step});
+      if (master) updated.push_back(master);
     }
     rs_adamw_opts o{number(a[7]), number(a[8]), number(a[9]), number(a[10]), 0.0};
     at::Tensor sumsq, norm;
@@ -481,11 +490,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         given_sumsq(sumsq, first);
       }
     }
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[6]); ++i) {
-      if (PyList_GET_ITEM(a[6], i) == Py_None) continue;
-      for (int list = 0; list < 5; ++list)
-        if (PyList_GET_ITEM(a[list], i) != Py_None) written(tensor(PyList_GET_ITEM(a[list], i), "a sub-field"));
-    }
+    for (const at::Tensor* x : updated) written(*x);  // here, since the lists may change while the lock is let go
     unlocked([&] {
       if (clip) norm = at::empty({}, first.options().dtype(at::kFloat));
       uint64_t bytes = 0;
