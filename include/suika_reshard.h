@@ -471,7 +471,7 @@ typedef struct rs_adamw_opts {
 
 /* step += 1 and one AdamW update of every tensor. With max_norm > 0 the gradients count times
  * min(1, max_norm / (norm + 1e-6)) without being written, and the norm goes to norm_dev (may be NULL): sqrt(*sumsq_dev)
- * where that is given, else the norm of these gradients. No two tensors may share memory. */
+ * where that is given, else the norm of these gradients (0 for no tensors). No two tensors may share memory. */
 int rs_adamw_workspace_bytes(int64_t n_tensors, uint64_t* bytes);
 int rs_adamw_step(const rs_adamw_tensor* tensors, int64_t n_tensors, const rs_adamw_opts* opts, const double* sumsq_dev,
                   float* norm_dev, void* workspace_dev, uint64_t workspace_bytes, int32_t device, void* stream);

@@ -622,7 +622,8 @@ extern "C" int rs_adamw_step(const rs_adamw_tensor* tensors, int64_t n, const rs
     if (!(o.beta1 >= 0 && o.beta1 < 1 && o.beta2 >= 0 && o.beta2 < 1 && o.eps >= 0 && o.lr >= 0))
       return tfail(RS_ERR_ARG, "rs_adamw_step: lr, betas or eps out of range");
     if (sumsq_dev ? !(o.max_norm > 0) : !(o.max_norm >= 0)) return tfail(RS_ERR_ARG, "rs_adamw_step: max_norm must be positive");
-    if (n == 0) return RS_OK;
+    const bool norm_alone = n == 0 && norm_dev && o.max_norm > 0;  // a rank without tensors
+    if (n == 0 && !norm_alone) return RS_OK;
     for (int64_t i = 0; i < n; ++i) {
       const rs_adamw_tensor& a = tensors[i];
       const std::string who = "rs_adamw_step: tensor " + std::to_string(i);
@@ -660,6 +661,7 @@ extern "C" int rs_adamw_step(const rs_adamw_tensor* tensors, int64_t n, const rs
       }
       partial = sums;
     }
+    if (norm_alone) return adam_chunk<16>(tensors, 0, o, partial, n_partial, norm_dev, scal, sms, st);
     for (int64_t i = 0; i < n; i += 560) {
       const int c = (int)std::min<int64_t>(n - i, 560);
       int rc = c <= 16 ? adam_chunk<16>(tensors + i, c, o, partial, n_partial, norm_dev, scal + i, sms, st)

@@ -1,5 +1,6 @@
 """The training-step operators at the edges of what their documentation allows, on a B200, against a plain
 computation in 64 bits where numbers are compared."""
+import ctypes
 import datetime
 import json
 import math
@@ -12,6 +13,7 @@ import traceback
 import pytest
 import torch
 
+from suika_b200 import _lib as L
 from suika_b200 import optimizer as OPT
 from suika_b200 import vocab as V
 from tests.test_gpu_training import (BF16, DEV, F32, HYPER, TYPES, U, assert_close, clone_state, gen, grads_of, half, make_state, randn,
@@ -232,6 +234,18 @@ def test_unequal_shards_over_a_group_find_their_places(monkeypatch, cuts, top):
             assert_close(r.logprob, whole.logprob, 500 * U * 12)
             if top:
                 assert torch.equal(r.top_index, whole.top_index)
+
+
+def test_update_entry_without_tensors_gives_the_norm():
+    lib, norm, ws = L.load(), torch.full((2,), 7.0, device=DEV), torch.zeros(1 << 20, dtype=torch.uint8, device=DEV)
+    sumsq = torch.full((1,), 25.0, dtype=torch.float64, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    for given, want in ((sumsq.data_ptr(), 5.0), (None, 0.0)):
+        o = L.RsAdamwOpts(1e-3, 0.9, 0.99, 1e-8, 1.0)
+        L.check(lib.rs_adamw_step(None, 0, ctypes.byref(o), given, norm.data_ptr(), ws.data_ptr(), ws.numel(), 0, stream))
+        assert norm.tolist() == [want, 7.0]
+    o = L.RsAdamwOpts(1e-3, 0.9, 0.99, 1e-8, 0.0)
+    L.check(lib.rs_adamw_step(None, 0, ctypes.byref(o), None, norm.data_ptr(), None, 0, 0, stream))  # no clipping, no norm
 
 
 # ---- tensors that autograd follows --------------------------------------------------------------
