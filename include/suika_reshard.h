@@ -424,7 +424,7 @@ int rs_act_resolve(const rs_stage_mesh* src, const rs_stage_mesh* dst, const rs_
  * lm_head shard's logits. Every entry launches on `stream` of `device` (any device may be current),
  * allocates nothing, waits for nothing and keeps nothing, so it can be captured into a CUDA graph.
  * Results do not depend on the order in which CTAs run. Workspaces are the caller's; calls that may run at the
- * same time need a workspace each. Element types: */
+ * same time need a workspace each, at a multiple of 256 bytes. Element types: */
 enum rs_dtype { RS_F32 = 0, RS_BF16 = 1, RS_F16 = 2 };
 
 /* One dense run of gradient elements that this rank counts. */

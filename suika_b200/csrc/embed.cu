@@ -542,12 +542,14 @@ int rs_embed_lookup(const rs_embed_opts* opts, const void* ids_dev, const void* 
 }
 
 int rs_embed_grad_workspace_bytes(const rs_embed_opts* opts, int32_t device, uint64_t* bytes) {
-  int rc = check_opts("rs_embed_grad_workspace_bytes", opts);
-  if (rc != RS_OK) return rc;
-  if (!bytes) return tfail(RS_ERR_ARG, "rs_embed_grad_workspace_bytes: NULL result");
-  if (opts->n_tokens > kSortMax) return tfail(RS_ERR_CAPACITY, "rs_embed_grad: more than 65536 tokens in one call");
-  *bytes = std::max<uint64_t>(256, plan_grad(*opts).bytes);
-  return RS_OK;
+  return guarded("rs_embed_grad_workspace_bytes", [&]() -> int {
+    int rc = check_opts("rs_embed_grad_workspace_bytes", opts);
+    if (rc != RS_OK) return rc;
+    if (!bytes) return tfail(RS_ERR_ARG, "rs_embed_grad_workspace_bytes: NULL result");
+    if (opts->n_tokens > kSortMax) return tfail(RS_ERR_CAPACITY, "rs_embed_grad: more than 65536 tokens in one call");
+    *bytes = std::max<uint64_t>(256, plan_grad(*opts).bytes);
+    return RS_OK;
+  });
 }
 
 int rs_embed_grad(const rs_embed_opts* opts, const void* ids_dev, const void* grad_out_dev, void* grad_dev, void* workspace,

@@ -799,7 +799,8 @@ int forward(const char* what, const rs_logprob_opts* o, const void* logits, cons
   const std::string w(what);
   if (!logits || !targets) return tfail(RS_ERR_ARG, w + ": NULL logits or targets");
   if (!record && (!logprob || !entropy || !lse || (o->top && (!top_value || !top_index)))) return tfail(RS_ERR_ARG, w + ": NULL output");
-  if ((uint64_t)logits % dtype_bytes(o->dtype) || (uint64_t)targets % (o->wide_targets ? 8 : 4))
+  if (misaligned(dtype_bytes(o->dtype), logits) || misaligned(o->wide_targets ? 8 : 4, targets) ||
+      misaligned(4, logprob, entropy, lse, top_value, record) || misaligned(8, top_index))
     return tfail(RS_ERR_ARG, w + ": an address is not aligned to its elements");
   DeviceGuard guard(device);
   if (guard.err != cudaSuccess) return tcuda(guard.err, (w + ": cudaSetDevice").c_str());
@@ -838,7 +839,8 @@ int backward(const char* what, const rs_logprob_opts* opts, int64_t first, int64
   const int b = dtype_bytes(o.dtype);
   if (!logits || !targets || !lse || !grad_logprob || !grad || (grad_entropy && !entropy))
     return tfail(RS_ERR_ARG, w + ": NULL address");
-  if ((uint64_t)logits % b || (uint64_t)grad % b || (uint64_t)targets % (o.wide_targets ? 8 : 4))
+  if (misaligned(b, logits, grad) || misaligned(o.wide_targets ? 8 : 4, targets) ||
+      misaligned(4, lse, entropy, grad_logprob, grad_entropy, grad_lse))
     return tfail(RS_ERR_ARG, w + ": an address is not aligned to its elements");
   if (o.n_rows > 1 && grad_stride < o.cols) return tfail(RS_ERR_ARG, w + ": the gradient's rows overlap");
   BwdArgs a{};
@@ -927,6 +929,8 @@ int rs_token_merge(const float* records_dev, const int64_t* starts, int32_t n_sh
     if (n_rows == 0) return RS_OK;
     if (!records_dev || !starts || !logprob_dev || !entropy_dev || !lse_dev || (top && (!top_logprob_dev || !top_index_dev)))
       return tfail(RS_ERR_ARG, "rs_token_merge: NULL address");
+    if (misaligned(4, records_dev, logprob_dev, entropy_dev, lse_dev, top_logprob_dev) || misaligned(8, top_index_dev))
+      return tfail(RS_ERR_ARG, "rs_token_merge: an address is not aligned to its elements");
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_token_merge: cudaSetDevice");
     FwdArgs a{};

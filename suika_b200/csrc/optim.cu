@@ -507,9 +507,11 @@ bool any_overlap(std::vector<std::pair<uint64_t, uint64_t>>& r) {
 extern "C" {
 
 int rs_grad_sumsq_workspace_bytes(int64_t n_spans, uint64_t* bytes) {
-  if (n_spans < 0 || !bytes) return tfail(RS_ERR_ARG, "rs_grad_sumsq_workspace_bytes: bad argument");
-  *bytes = partial_bytes(n_spans);
-  return RS_OK;
+  return guarded("rs_grad_sumsq_workspace_bytes", [&]() -> int {
+    if (n_spans < 0 || !bytes) return tfail(RS_ERR_ARG, "rs_grad_sumsq_workspace_bytes: bad argument");
+    *bytes = partial_bytes(n_spans);
+    return RS_OK;
+  });
 }
 
 int rs_grad_sumsq(const rs_grad_span* spans, int64_t n, void* workspace, uint64_t workspace_bytes, double* sumsq_dev,
@@ -518,10 +520,11 @@ int rs_grad_sumsq(const rs_grad_span* spans, int64_t n, void* workspace, uint64_
     std::vector<rs_grad_span> s;
     int rc = check_spans("rs_grad_sumsq", spans, n, &s);
     if (rc != RS_OK) return rc;
-    if (!sumsq_dev) return tfail(RS_ERR_ARG, "rs_grad_sumsq: NULL result");
+    if (!sumsq_dev || misaligned(8, sumsq_dev)) return tfail(RS_ERR_ARG, "rs_grad_sumsq: NULL or misaligned result");
     uint64_t need = 0;
     rs_grad_sumsq_workspace_bytes((int64_t)s.size(), &need);
-    if (!workspace || workspace_bytes < need) return tfail(RS_ERR_CAPACITY, "rs_grad_sumsq: workspace too small");
+    if (!workspace || workspace_bytes < need || misaligned(8, workspace))
+      return tfail(RS_ERR_CAPACITY, "rs_grad_sumsq: workspace too small or not 8-byte aligned");
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return tcuda(guard.err, "rs_grad_sumsq: cudaSetDevice");
     const int sms = std::min(sm_count(device), kMaxSms);
@@ -556,6 +559,7 @@ int rs_grad_clip(const rs_grad_span* spans, int64_t n, const double* sumsq_dev, 
     int rc = check_spans("rs_grad_clip", spans, n, &s);
     if (rc != RS_OK) return rc;
     if (!sumsq_dev || !norm_dev) return tfail(RS_ERR_ARG, "rs_grad_clip: NULL sum of squares or norm");
+    if (misaligned(8, sumsq_dev) || misaligned(4, norm_dev)) return tfail(RS_ERR_ARG, "rs_grad_clip: a misaligned sum of squares or norm");
     if (!(max_norm > 0.f)) return tfail(RS_ERR_ARG, "rs_grad_clip: max_norm must be positive");
     std::vector<std::pair<uint64_t, uint64_t>> ranges;
     ranges.reserve(s.size());
@@ -576,9 +580,11 @@ int rs_grad_clip(const rs_grad_span* spans, int64_t n, const double* sumsq_dev, 
 }
 
 int rs_adamw_workspace_bytes(int64_t n_tensors, uint64_t* bytes) {
-  if (n_tensors < 0 || !bytes) return tfail(RS_ERR_ARG, "rs_adamw_workspace_bytes: bad argument");
-  *bytes = (std::max<uint64_t>(1, (uint64_t)n_tensors) * sizeof(float4) + 255) / 256 * 256 + partial_bytes(n_tensors);
-  return RS_OK;
+  return guarded("rs_adamw_workspace_bytes", [&]() -> int {
+    if (n_tensors < 0 || !bytes) return tfail(RS_ERR_ARG, "rs_adamw_workspace_bytes: bad argument");
+    *bytes = (std::max<uint64_t>(1, (uint64_t)n_tensors) * sizeof(float4) + 255) / 256 * 256 + partial_bytes(n_tensors);
+    return RS_OK;
+  });
 }
 
 }  // extern "C"
@@ -622,6 +628,7 @@ extern "C" int rs_adamw_step(const rs_adamw_tensor* tensors, int64_t n, const rs
     if (!(o.beta1 >= 0 && o.beta1 < 1 && o.beta2 >= 0 && o.beta2 < 1 && o.eps >= 0 && o.lr >= 0))
       return tfail(RS_ERR_ARG, "rs_adamw_step: lr, betas or eps out of range");
     if (sumsq_dev ? !(o.max_norm > 0) : !(o.max_norm >= 0)) return tfail(RS_ERR_ARG, "rs_adamw_step: max_norm must be positive");
+    if (misaligned(8, sumsq_dev) || misaligned(4, norm_dev)) return tfail(RS_ERR_ARG, "rs_adamw_step: a misaligned sum of squares or norm");
     const bool norm_alone = n == 0 && norm_dev && o.max_norm > 0;  // a rank without tensors
     if (n == 0 && !norm_alone) return RS_OK;
     for (int64_t i = 0; i < n; ++i) {

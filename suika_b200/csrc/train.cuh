@@ -54,6 +54,12 @@ inline int sm_count(int device) {
 inline int dtype_bytes(uint32_t dtype) { return dtype == RS_F32 ? 4 : 2; }
 inline bool dtype_known(uint32_t dtype) { return dtype <= RS_F16; }
 
+// Whether one of the addresses does not lie at a multiple of `bytes` (NULL does).
+template <class... P>
+bool misaligned(int bytes, P... p) {
+  return (((uint64_t)p % bytes != 0) || ...);
+}
+
 // Runs `body` so that no C++ exception leaves a C entry.
 template <class F>
 int guarded(const char* what, F&& body) {

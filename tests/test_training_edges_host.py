@@ -1,6 +1,7 @@
 """Refusals of the training-step operators that are made before any CUDA call."""
 import ctypes
 
+import numpy as np
 import torch
 
 from suika_b200 import _lib as L
@@ -62,3 +63,32 @@ def test_embedding_gradient_of_long_batches_refuses_its_own_input():
                 meet = _rows_meet(40, n, stride, hidden, at, out_rows * hidden)
                 assert V._touches(g, out) == meet, (n, stride, hidden, out_rows, at)
     assert not V._touches(whole[:0].view(0, 4), whole[:8].view(2, 4)) and not V._touches(whole[:8].view(2, 4), whole[:0].view(0, 4))
+
+
+def test_entries_refuse_misaligned_addresses():
+    """Statistics, results and workspaces are 4 or 8 bytes wide: an address between two of them would fault on the device."""
+    lib = L.load()
+    span = np.array([(FAKE, 4, L.RS_F32, 0)], dtype=L.GRAD_SPAN_DTYPE)
+    assert lib.rs_grad_sumsq(span.ctypes.data, 1, FAKE + 4, 1 << 20, FAKE, 0, None) == L.RS_ERR_CAPACITY
+    assert lib.rs_grad_sumsq(span.ctypes.data, 1, FAKE, 1 << 20, FAKE + 4, 0, None) == L.RS_ERR_ARG
+    assert lib.rs_grad_clip(span.ctypes.data, 1, FAKE + 4, 1.0, FAKE, 0, None) == L.RS_ERR_ARG
+    assert lib.rs_grad_clip(span.ctypes.data, 1, FAKE, 1.0, FAKE + 2, 0, None) == L.RS_ERR_ARG
+    adam = np.array([(FAKE,) * 6 + (4, 0.0, 0, 0, 0)], dtype=L.ADAMW_TENSOR_DTYPE)
+    opts = L.RsAdamwOpts(1e-3, 0.9, 0.99, 1e-8, 1.0)
+    for sumsq, norm in ((FAKE + 4, FAKE), (FAKE, FAKE + 2)):
+        assert lib.rs_adamw_step(adam.ctypes.data, 1, ctypes.byref(opts), sumsq, norm, FAKE, 1 << 20, 0, None) == L.RS_ERR_ARG
+        assert b"misaligned" in lib.rs_last_error()
+    o = L.RsLogprobOpts(4, 8, 8, 0, L.RS_F32, 1, 2, 0)
+    outs = [FAKE] * 5
+    for i in range(5):
+        bad = list(outs)
+        bad[i] += 2 if i < 4 else 4
+        assert lib.rs_token_logprobs(ctypes.byref(o), FAKE, FAKE, *bad, 0, None) == L.RS_ERR_ARG and b"aligned" in lib.rs_last_error()
+        starts = np.zeros(1, np.int64)
+        assert lib.rs_token_merge(FAKE, starts.ctypes.data, 1, 4, 2, *bad, 0, None) == L.RS_ERR_ARG and b"aligned" in lib.rs_last_error()
+    assert lib.rs_token_merge(FAKE + 2, starts.ctypes.data, 1, 4, 2, *outs, 0, None) == L.RS_ERR_ARG
+    assert lib.rs_token_record(ctypes.byref(o), FAKE, FAKE, FAKE + 2, 0, None) == L.RS_ERR_ARG
+    for i in range(5):
+        bad = list(outs)
+        bad[i] += 2
+        assert lib.rs_token_logprobs_grad(ctypes.byref(o), FAKE, FAKE, *bad, FAKE, 8, 0, None) == L.RS_ERR_ARG and b"aligned" in lib.rs_last_error()
