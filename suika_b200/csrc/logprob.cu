@@ -5,9 +5,10 @@
 // A = sum of e^(z - m) (z - m), rescaled where m grows; then lse = m + log S and the entropy is
 // log S - A / S. The differences z - m are taken first, so logits of any size (the type's lowest
 // value as a mask among them) neither overflow nor lose the digits that the exponent needs. The
-// top alternatives need no second pass over the row: each thread notes the maximum of every 64
-// bytes it reads, the k-th largest maximum of 64 groups of threads is a bound that at least k logits reach (44 do for
-// k = 32, fewer for less), and only the noted places that reach it are read again. All sums are in 32 bits.
+// top alternatives need no second pass over the row: each thread notes up to 16 maxima, of 64 bytes that it
+// reads each (or of more where it reads more than 1 KB), the k-th largest maximum of 64 groups of threads is a
+// bound that at least k logits reach (44 do for k = 32, fewer for less), and only the noted places that reach
+// it are read again. All sums are in 32 bits.
 //
 // HBM is the bound for many rows (each logit is read once, the gradient reads and writes once).
 // Few rows are split over the CTAs of a cluster, which join through distributed shared memory.
@@ -755,10 +756,7 @@ int launch_forward_as(FwdArgs a, int cs, cudaStream_t st) {
     const int64_t its = ((vecs + cs - 1) / cs + 1 + kUnroll * THREADS - 1) / (kUnroll * THREADS);
     a.per_note = (int)((its + kNotes - 1) / kNotes);
     smem = (size_t)((its + a.per_note - 1) / a.per_note) * THREADS * sizeof(float);
-    if (smem > 32 * 1024) {  // with the static arrays, past the 48 KB that need no opt-in
-      cudaError_t e = cudaFuncSetAttribute(forward_kernel<T, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return tcuda(e, "rs_token_logprobs: cudaFuncSetAttribute");
-    }
+    static_assert(kNotes * THREADS * 4 + kMaxCand * 8 + kMaxHits * 4 + 4096 <= 48 * 1024, "the notes and the static arrays need no opt-in");
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.n * cs));
