@@ -897,8 +897,8 @@ def run_checkpoint(args):
 def run_next_step(args):
     """The step a job takes after its reshard: cfg2b on a layer sample (every target rank's state on one GPU, resharded by
     reshard_local), then, per rank, the global gradient norm (each replicated tensor counted once), clipping and
-    AdamW on the master with bf16 gradients. Beside it torch's own: clip_grad_norm_ and AdamW(foreach) on the
-    masters and fp32 gradients, then the bf16 parameters copied from the masters. Device time, CUDA events; the
+    AdamW on the master with bf16 gradients. Beside it torch's own: clip_grad_norm_ and AdamW, fused (its one-pass form)
+    and foreach, on the masters and fp32 gradients, then the bf16 parameters copied from the masters. Device time, CUDA events; the
     state and gradients are larger than L2."""
     from suika_b200 import optimizer as OPT
     dev = torch.device("cuda", 0)
@@ -921,19 +921,23 @@ def run_next_step(args):
     params = [torch.nn.Parameter(e["master"]) for st in states.values() for e in st.values()]
     for p, g in zip(params, (g for gs in grads.values() for g in gs.values())):
         p.grad = g.float()
-    adam = torch.optim.AdamW(params, lr=1e-4, weight_decay=0.1, foreach=True)
     bf16 = [e["param"] for st in states.values() for e in st.values()]
 
-    def torchs():
-        torch.nn.utils.clip_grad_norm_(params, 1.0, foreach=True)
-        adam.step()
-        torch._foreach_copy_(bf16, [p.detach() for p in params])
-    t_torch = _median_event_s(torchs, args.steps)
+    def torchs(**form):
+        adam = torch.optim.AdamW(params, lr=1e-4, weight_decay=0.1, **form)
+
+        def step():
+            torch.nn.utils.clip_grad_norm_(params, 1.0, foreach=True)
+            adam.step()
+            torch._foreach_copy_(bf16, [p.detach() for p in params])
+        return _median_event_s(step, args.steps)
+    t_fused, t_foreach = torchs(fused=True), torchs(foreach=True)
     nbytes = elements * (2 + 12 + 12 + 2)
     return {"metric": "clipped AdamW update of a resharded training state", "value": round(nbytes / t_ours / 1e9, 1), "unit": "GB/s",
             "n_gpus": 1, "steps": args.steps, "ms_per_step": round(t_ours * 1e3, 3), "higher_is_better": True, "data": "synthetic",
             "config": {"workload": f"{cfg.note}, {cfg.spec.n_layers} layers, both target ranks on one GPU; bf16 gradients, fp32 master and moments"},
-            "elements": elements, "torch_foreach_ms_per_step": round(t_torch * 1e3, 3), "speedup": round(t_torch / t_ours, 2)}
+            "elements": elements, "torch_fused_ms_per_step": round(t_fused * 1e3, 3), "torch_foreach_ms_per_step": round(t_foreach * 1e3, 3),
+            "speedup": round(t_fused / t_ours, 2)}
 
 
 # ---------------------------------------------------------------------------------------------

@@ -238,9 +238,10 @@ __device__ __forceinline__ void store_out(G* out, int64_t at, const float* x) {
 // tokens is summed whole by the tile where it starts (up to 15 tokens of the next tile are read); a
 // longer one is cut at the tiles' borders, and its pieces go to `partial` for the join. So no warp sums more than
 // 31 tokens, however uneven the ids are. The keys from one tile before to one after are held
-// two to a lane; where rows start is one 64-bit mask; warps need no barrier. Tokens are taken one by one:
-// two or four in flight per warp cost the registers of more warps than they are worth (30011 tokens of 3584 columns added to
-// an fp32 gradient: 155 us, 174 and 209).
+// two to a lane; where rows start is one 64-bit mask; warps need no barrier. Tokens are taken one by one: two or
+// four in flight per warp cost the registers of more warps than they are worth (30011 tokens of 3584 columns added
+// to an fp32 gradient, the whole gradient when these three were compared: 155 us, 174 and 209; now 122 with cold
+// caches). That is a size with warps to spare: 8192 tokens of which half are held leave some idle.
 template <class T, class G, int E, bool ACC>
 __global__ void __launch_bounds__(256) sum_kernel(SumArgs a, const T* grad, G* out, int64_t units) {
   let_successor_start();

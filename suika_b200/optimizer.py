@@ -215,7 +215,8 @@ class ShardAdamW:
             raise ValueError("sub-fields of the state share memory")
 
     def step(self, grads: Dict[str, torch.Tensor], *, sumsq: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
-        """One update from {name: gradient}; names without a gradient (missing or None) stay as they are.
+        """One update from {name: gradient}; names without a gradient (missing or None) stay as they are, and
+        gradients share no memory with the state.
         Returns the norm before clipping (float32, on the device), or None without max_norm. `sumsq`:
         the global sum of squares, if the caller has it already. With a group, or a given sumsq, there may be
         no gradient at all: the rank takes part in the sum and nothing is updated."""
