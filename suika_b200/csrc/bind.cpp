@@ -44,7 +44,8 @@ void raise_status(int rc) {
 }
 
 // Allocation and launches run in `body` without the interpreter's lock: a full launch queue or a cudaMalloc
-// waits in the driver, and other Python threads go on. Nothing of Python is touched in there.
+// waits in the driver, and other Python threads go on. Nothing of Python is touched in there; the arguments' own
+// references, and for lists of tensors those of the caller's lists, keep the tensors until the call returns.
 template <class F>
 auto unlocked(F&& body) {
   struct Unlock {
@@ -406,7 +407,7 @@ PyObject* grad_sumsq(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const auto ts = tensors_of(a[0], "gradients");
     const auto s = spans_of(ts);
-    const at::Tensor first = *ts[0];  // the list may change meanwhile
+    const at::Tensor& first = *ts[0];
     return THPVariable_Wrap(unlocked([&] { return sumsq_of(s, first); }));
   });
 }
@@ -417,16 +418,16 @@ PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
     count_args("grad_clip", n, 3);
     const auto ts = tensors_of(a[0], "gradients");
     const auto s = spans_of(ts);
-    const at::Tensor first = *ts[0];
+    const at::Tensor& first = *ts[0];
     const float max_norm = (float)number(a[1]);
     at::Tensor sumsq;
     if (a[2] != Py_None) sumsq = tensor(a[2], "sumsq");
-    for (const at::Tensor* t : ts) written(*t);  // here, since the list may change while the lock is let go
     return THPVariable_Wrap(unlocked([&] {
       if (!sumsq.defined()) sumsq = sumsq_of(s, first);
       at::Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
       check(rs_grad_clip(s.data(), (int64_t)s.size(), given_sumsq(sumsq, first), max_norm, norm.data_ptr<float>(), first.get_device(),
                          stream_of(first)));
+      for (const at::Tensor* t : ts) written(*t);
       return norm;
     }));
   });
@@ -441,7 +442,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (int i = 0; i < 7; ++i)
       if (!PyList_Check(a[i]) || PyList_GET_SIZE(a[i]) != PyList_GET_SIZE(a[0])) throw Raise{PyExc_TypeError, "lists of one length are taken"};
     const auto ts = tensors_of(a[6], "gradients");
-    const at::Tensor first = *ts[0];
+    const at::Tensor& first = *ts[0];
     const double decay = number(a[11]);
     std::vector<rs_adamw_tensor> t;
     std::vector<const at::Tensor*> updated;
@@ -490,7 +491,6 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         given_sumsq(sumsq, first);
       }
     }
-    for (const at::Tensor* x : updated) written(*x);  // here, since the lists may change while the lock is let go
     unlocked([&] {
       if (clip) norm = at::empty({}, first.options().dtype(at::kFloat));
       uint64_t bytes = 0;
@@ -498,6 +498,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const at::Tensor workspace = at::empty({(int64_t)bytes}, first.options().dtype(at::kByte));
       check(rs_adamw_step(t.data(), (int64_t)t.size(), &o, sumsq.defined() ? sumsq.data_ptr<double>() : nullptr,
                           clip ? norm.data_ptr<float>() : nullptr, workspace.data_ptr(), bytes, first.get_device(), stream_of(first)));
+      for (const at::Tensor* x : updated) written(*x);
     });
     return clip ? THPVariable_Wrap(std::move(norm)) : Py_NewRef(Py_None);
   });

@@ -272,6 +272,23 @@ def test_what_is_written_in_place_counts_as_written():
     assert z._version > v
 
 
+def test_a_refused_call_counts_as_nothing_written():
+    x = torch.zeros(100, device=DEV)
+    v = x._version
+    with pytest.raises(RuntimeError, match="share memory"):
+        OPT.clip_grads([x[:60], x[50:]], 1.0)
+    state = make_state([100, 7], BF16, F32, True)
+    before = {n: {s: t._version for s, t in e.items()} for n, e in state.items()}
+    opt = OPT.ShardAdamW(state, **HYPER)
+    for grads in ({"t0": torch.zeros(100, device=DEV), "t1": torch.zeros(8, device=DEV)}, {"t0": torch.zeros(200, device=DEV)[::2]}):
+        with pytest.raises((AssertionError, ValueError)):
+            opt.step(grads)
+    opt.lr = -1.0
+    with pytest.raises(RuntimeError, match="out of range"):
+        opt.step({"t0": torch.zeros(100, device=DEV)})
+    assert x._version == v and before == {n: {s: t._version for s, t in e.items()} for n, e in state.items()}
+
+
 def test_a_backward_pass_over_what_was_written_is_an_error():
     state = make_state([12], F32, F32, False)
     w = state["t0"]["param"].requires_grad_()
